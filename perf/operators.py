@@ -361,7 +361,8 @@ def _update(s):
     copied = (grow > 0) & (length % page != 0) & (refs[last.clamp(min=0)] > 1)
     longer = length + grow
     wanted = (longer + page - 1) // page
-    need = wanted - count + copied
+    copied &= wanted <= cols
+    need = torch.where(wanted > cols, 0, wanted - count + copied)
     free = refs == 0
     missing = need.sum() - free.sum()
     wide = (wanted > cols).sum()
