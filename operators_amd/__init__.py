@@ -15,8 +15,13 @@ from .liboperators import (  # noqa: F401
     infiniopAttentionDescriptor_t,
     infiniopCausalSoftmaxDescriptor_t,
     infiniopHandle_t,
+    infiniopKVCacheAppendDescriptor_t,
+    infiniopKVCacheCopyDescriptor_t,
     infiniopMatmulDescriptor_t,
     infiniopMLPDescriptor_t,
+    infiniopPagedAttentionDescriptor_t,
+    infiniopPageTableCompactDescriptor_t,
+    infiniopPageTableUpdateDescriptor_t,
     infiniopRearrangeDescriptor_t,
     infiniopRMSNormDescriptor_t,
     infiniopRandomSampleDescriptor_t,
@@ -24,6 +29,7 @@ from .liboperators import (  # noqa: F401
     infiniopSwiGLUDescriptor_t,
     infiniopTensorDescriptor_t,
     open_lib,
+    open_paged_lib,
 )
 from .utils import (  # noqa: F401
     InfiniopError,

@@ -1,4 +1,4 @@
-"""Build libinfiniop.so (amd-gpu device, gfx950 only) with hipcc.
+"""Build libinfiniop.so and libinfiniop_paged.so (amd-gpu device, gfx950 only) with hipcc.
 
     python -m operators_amd.build            # compile everything, link in-tree
     python -m operators_amd.build --install  # also copy lib + headers to $INFINI_ROOT
@@ -24,6 +24,10 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libinfiniop.so")
+# the operators of the paged cache, which the reference does not have: a library of their own, so that
+# libinfiniop.so exports the reference's entry points and nothing else
+PAGED = os.path.join(CSRC, "paged")
+PAGED_LIB_PATH = os.path.join(LIB_DIR, "libinfiniop_paged.so")
 
 ARCH = "gfx950"
 
@@ -122,7 +126,7 @@ def build(verbose=True, jobs=None):
     os.makedirs(LIB_DIR, exist_ok=True)
     srcs = sources()
     jobs = jobs or min(8, os.cpu_count() or 1)
-    objs, resources = [], {}
+    objs, resources = {LIB_PATH: [], PAGED_LIB_PATH: []}, {}
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
         for src, obj, rc, err, res_of in pool.map(_compile, srcs):
             if verbose:
@@ -131,7 +135,7 @@ def build(verbose=True, jobs=None):
                 print(err, file=sys.stderr)
             if rc != 0:
                 raise RuntimeError(f"compilation failed: {src}")
-            objs.append(obj)
+            objs[PAGED_LIB_PATH if src.startswith(PAGED + os.sep) else LIB_PATH].append(obj)
             for name, fig in res_of.items():
                 resources[name] = dict(fig, source=os.path.relpath(src, REPO_DIR))
     names = sorted(resources)
@@ -145,13 +149,14 @@ def build(verbose=True, jobs=None):
         raise RuntimeError(f"{len(spilling)} kernels spill vector registers to scratch memory (see {RESOURCES_PATH})")
     if verbose:
         print(f"[resources] {len(record)} kernels, none spills; {os.path.relpath(RESOURCES_PATH, REPO_DIR)}", flush=True)
-    cmd = [hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", LIB_PATH] + objs
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        print(res.stderr, file=sys.stderr)
-        raise RuntimeError("link failed")
-    if verbose:
-        print(f"[link] {os.path.relpath(LIB_PATH, REPO_DIR)}", flush=True)
+    for path, parts in objs.items():
+        cmd = [hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", path] + parts
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            print(res.stderr, file=sys.stderr)
+            raise RuntimeError("link failed")
+        if verbose:
+            print(f"[link] {os.path.relpath(path, REPO_DIR)}", flush=True)
     return LIB_PATH
 
 
@@ -176,10 +181,11 @@ def build_c_client(verbose=True):
 
 
 def install(root):
-    """Copy the library and headers where the reference's loader looks
+    """Copy the libraries and headers where the reference's loader looks
     ($INFINI_ROOT/lib/libinfiniop.so, operatorspy/liboperators.py:11,55)."""
     os.makedirs(os.path.join(root, "lib"), exist_ok=True)
-    shutil.copy2(LIB_PATH, os.path.join(root, "lib", "libinfiniop.so"))
+    for path in (LIB_PATH, PAGED_LIB_PATH):
+        shutil.copy2(path, os.path.join(root, "lib", os.path.basename(path)))
     shutil.copytree(INCLUDE, os.path.join(root, "include"), dirs_exist_ok=True)
 
 

@@ -1,0 +1,69 @@
+// Device side of page_table.h.  Include from .hip files only.
+#ifndef INFINIOP_AMD_PAGE_TABLE_KERNEL_H
+#define INFINIOP_AMD_PAGE_TABLE_KERNEL_H
+
+#include "page_table.h"
+#include "paged_kernel.h"
+
+namespace amd {
+
+// A phase of one of these operators is written for `count` workgroups of which
+// this is number `index`, so that it may be a launch of its own or a part of one.
+struct Crew {
+    uint32_t index, count;
+};
+
+// What one phase wrote to memory, plainly or by atomics, to the next phase in the same workgroup.
+__device__ __forceinline__ void phase_end() {
+    __threadfence();
+    __syncthreads();
+}
+
+// The bits of `test(page)` for all pages of the crew's chunks, and how many are set in each chunk.
+template<int WAVES, typename F>
+__device__ __forceinline__ void mark_pages(Crew crew, uint32_t pages, uint64_t *words, uint32_t *counts, uint32_t *slots, F test) {
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t chunks = (pages + kChunkPages - 1) / kChunkPages;
+    for (uint32_t c = crew.index; c < chunks; c += crew.count) {
+        uint32_t set = 0;
+        for (uint32_t w = wave; w < kChunkWords; w += WAVES) {
+            const uint32_t p = c * kChunkPages + w * 64 + lane;
+            const uint64_t bits = __builtin_amdgcn_ballot_w64(p < pages && test(p));
+            if (lane == 0) words[c * kChunkWords + w] = bits;
+            set += static_cast<uint32_t>(__builtin_popcountll(bits));
+        }
+        if (lane == 0) slots[wave] = set;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t all = 0;
+            for (int i = 0; i < WAVES; ++i) all += slots[i];
+            counts[c] = all;
+        }
+        __syncthreads();
+    }
+}
+
+// The sum of counts[0 .. upto) and of counts[0 .. chunks), to every lane of the workgroup.
+template<int WAVES>
+__device__ __forceinline__ void count_before(const uint32_t *counts, uint32_t upto, uint32_t chunks, uint64_t *slots, uint32_t *before, uint32_t *all) {
+    uint64_t both = 0, total;// low half: all, high half: before
+    for (uint32_t c = threadIdx.x; c < chunks; c += WAVES * kWave) {
+        const uint64_t n = counts[c];
+        both += n | (c < upto ? n << 32 : 0);
+    }
+    block_scan64<WAVES>(both, slots, &total);
+    *all = static_cast<uint32_t>(total);
+    *before = static_cast<uint32_t>(total >> 32);
+}
+
+// How many bits of the chunk's words lie below bit `page` of it.
+__device__ __forceinline__ uint32_t bits_below(const uint64_t *words, uint32_t page) {
+    const uint32_t word = page / 64, first = page / kChunkPages * kChunkWords;
+    uint32_t n = 0;
+    for (uint32_t w = first; w < word; ++w) n += static_cast<uint32_t>(__builtin_popcountll(words[w]));
+    return n + static_cast<uint32_t>(__builtin_popcountll(words[word] & ((1ull << (page & 63)) - 1)));
+}
+
+}// namespace amd
+
+#endif

@@ -1,0 +1,231 @@
+// gfx950 PageTableUpdate: which row holds which pages after a step.
+//     rows:    row r := row source[r]; refcount[p] += rows that got p - rows that gave it up
+//     growth:  need[r] = pages(length + grow) - pages(length) + (1 if the last page is shared and grows)
+//     fresh:   the k-th free page goes to the row whose need covers k in the running sum
+// Four phases, each of which needs all of the one before: (1) the rows that change
+// are laid aside, (2) counts, (3) free pages marked and counted, needs worked out,
+// rows written, (4) fresh pages handed out.  Whole numbers throughout, added by
+// atomics whose order does not matter.  Latency bound: small tables go through the
+// phases in one workgroup and one launch, larger ones in four launches.
+#include "../../page_table_kernel.h"
+#include "page_table_update_amd.h"
+
+namespace {
+
+using namespace amd;
+
+constexpr int kTableWaves = 4, kOneWaves = 16;// per workgroup: of four launches, of one
+// a row's growth: its pages, and whether the first of them takes the place of the last page
+constexpr uint32_t kCopies = 1u << 31, kTooWide = 1u << 30;
+
+struct UpdateArgs {
+    const int *table, *lengths, *refcount, *source, *grow;
+    int *new_table, *new_lengths, *new_refcount, *pairs, *result;
+    int64_t stride, new_stride;
+    uint32_t rows, cols, pages, page;
+    FastDiv by_page;
+    // workspace
+    uint64_t *words;
+    uint32_t *counts, *before, *need;// free pages by chunk; lengths before growth; growth
+    int *aside;                      // [rows, cols]
+};
+
+__device__ __forceinline__ uint32_t in_range(const UpdateArgs &a, int length) {
+    const uint32_t room = a.cols * a.page;// < 2^31
+    return length < 0 ? 0 : static_cast<uint32_t>(length) > room ? room : static_cast<uint32_t>(length);
+}
+__device__ __forceinline__ uint32_t pages_of(const UpdateArgs &a, uint32_t tokens) { return fast_quotient(tokens + a.page - 1, a.by_page); }
+__device__ __forceinline__ bool changes(const UpdateArgs &a, uint32_t r) { return a.source[r] != static_cast<int>(r); }
+
+// (1) rows that change, laid aside; lengths before growth; the counts, where they go elsewhere
+template<int WAVES>
+__device__ void lay_aside(const UpdateArgs &a, Crew crew) {
+    const uint32_t lanes = WAVES * kWave;
+    for (uint32_t r = crew.index; r < a.rows; r += crew.count) {
+        const uint32_t s = static_cast<uint32_t>(a.source[r]);
+        const uint32_t length = s < a.rows ? in_range(a, a.lengths[s]) : 0, n = pages_of(a, length);
+        if (threadIdx.x == 0) a.before[r] = length;
+        if (s == r) continue;
+        for (uint32_t c = threadIdx.x; c < a.cols; c += lanes) a.aside[static_cast<uint64_t>(r) * a.cols + c] = c < n ? a.table[s * a.stride + c] : -1;
+    }
+    if (a.new_refcount != a.refcount) {
+        for (uint64_t p = static_cast<uint64_t>(crew.index) * lanes + threadIdx.x; p < a.pages; p += static_cast<uint64_t>(crew.count) * lanes)
+            a.new_refcount[p] = a.refcount[p];
+    }
+}
+
+// (2) what rows got, and what they gave up
+template<int WAVES>
+__device__ void count_rows(const UpdateArgs &a, Crew crew) {
+    const uint32_t lanes = WAVES * kWave;
+    for (uint32_t r = crew.index; r < a.rows; r += crew.count) {
+        if (!changes(a, r)) continue;
+        const uint32_t had = pages_of(a, in_range(a, a.lengths[r])), has = pages_of(a, a.before[r]);
+        for (uint32_t c = threadIdx.x; c < had; c += lanes) {
+            const uint32_t p = static_cast<uint32_t>(a.table[r * a.stride + c]);
+            if (p < a.pages) atomicAdd(a.new_refcount + p, -1);
+        }
+        for (uint32_t c = threadIdx.x; c < has; c += lanes) {
+            const uint32_t p = static_cast<uint32_t>(a.aside[static_cast<uint64_t>(r) * a.cols + c]);
+            if (p < a.pages) atomicAdd(a.new_refcount + p, 1);
+        }
+    }
+}
+
+// (3) free pages, needs, rows without their growth
+template<int WAVES>
+__device__ void work_out(const UpdateArgs &a, Crew crew, uint32_t *slots) {
+    const uint32_t lanes = WAVES * kWave;
+    mark_pages<WAVES>(crew, a.pages, a.words, a.counts, slots, [&](uint32_t p) { return a.new_refcount[p] == 0; });
+    for (uint32_t r = crew.index; r < a.rows; r += crew.count) {
+        const bool changed = changes(a, r);
+        const int *row = changed ? a.aside + static_cast<uint64_t>(r) * a.cols : a.table + r * a.stride;
+        if (threadIdx.x == 0) {
+            const uint32_t length = a.before[r], has = pages_of(a, length);
+            const uint32_t by = a.grow[r] > 0 ? static_cast<uint32_t>(a.grow[r]) : 0;
+            uint32_t need = kTooWide;
+            if (by <= a.cols * a.page - length) {
+                need = pages_of(a, length + by) - has;
+                if (by != 0 && has * a.page != length) {
+                    const uint32_t last = static_cast<uint32_t>(row[has - 1]);
+                    if (last < a.pages && a.new_refcount[last] > 1) need = (need + 1) | kCopies;
+                }
+            }
+            a.need[r] = need;
+            a.pairs[2 * r] = -1;
+            a.pairs[2 * r + 1] = -1;
+        }
+        if (changed || a.new_table != a.table) {
+            for (uint32_t c = threadIdx.x; c < a.cols; c += lanes) a.new_table[r * a.new_stride + c] = row[c];
+        }
+    }
+}
+
+// (4) fresh pages to the rows that grow.  ends: LDS, for each row the sum of the needs up to it and its own.
+template<int WAVES>
+__device__ void hand_out(const UpdateArgs &a, Crew crew, uint32_t *ends, uint64_t *slots) {
+    const uint32_t lanes = WAVES * kWave, chunks = (a.pages + kChunkPages - 1) / kChunkPages;
+    const uint32_t run = (a.rows + lanes - 1) / lanes, r0 = threadIdx.x * run;
+    uint64_t mine = 0, total, wide = 0, all_wide;
+    for (uint32_t r = r0; r < r0 + run && r < a.rows; ++r) {
+        const uint32_t n = a.need[r];
+        if (n == kTooWide) wide += 1;
+        else mine += n & ~kCopies;
+    }
+    uint64_t at = block_scan64<WAVES>(mine, slots, &total);
+    block_scan64<WAVES>(wide, slots, &all_wide);
+    for (uint32_t r = r0; r < r0 + run && r < a.rows; ++r) {
+        const uint32_t n = a.need[r];
+        at += n == kTooWide ? 0 : n & ~kCopies;
+        ends[r] = static_cast<uint32_t>(at);// (sums beyond 2^32 do not fit into the pages, and nothing is handed out)
+    }
+    uint32_t unused, all_free;
+    count_before<WAVES>(a.counts, 0, chunks, slots, &unused, &all_free);
+    const bool fits = all_wide == 0 && total <= all_free;
+    __syncthreads();
+    for (uint32_t r = crew.index * lanes + threadIdx.x; r < a.rows; r += crew.count * lanes) {
+        a.new_lengths[r] = static_cast<int>(a.before[r] + (fits && a.grow[r] > 0 ? a.grow[r] : 0));
+    }
+    if (crew.index == 0 && threadIdx.x == 0) {
+        const uint64_t lacks = total > all_free ? total - all_free : 0;
+        a.result[0] = lacks > 0x7FFFFFFF ? 0x7FFFFFFF : static_cast<int>(lacks);
+        a.result[1] = static_cast<int>(all_wide);
+    }
+    if (!fits) return;// (uniform over the workgroup)
+    for (uint32_t c = crew.index; c < chunks; c += crew.count) {
+        uint32_t base;
+        count_before<WAVES>(a.counts, c, chunks, slots, &base, &unused);
+        if (base >= total) break;
+        for (uint32_t i = threadIdx.x; i < kChunkPages; i += lanes) {
+            const uint32_t p = c * kChunkPages + i;
+            if (((a.words[c * kChunkWords + i / 64] >> (i & 63)) & 1) == 0) continue;
+            const uint32_t k = base + bits_below(a.words, p);
+            if (k >= total) continue;
+            uint32_t lo = 0, hi = a.rows - 1;// the first row whose needs end beyond k
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (ends[mid] > k) hi = mid;
+                else lo = mid + 1;
+            }
+            const uint32_t need = a.need[lo], nth = k - (ends[lo] - (need & ~kCopies)), has = pages_of(a, a.before[lo]);
+            int *row = a.new_table + lo * a.new_stride;
+            a.new_refcount[p] = 1;
+            if ((need & kCopies) != 0 && nth == 0) {
+                const int last = row[has - 1];
+                a.pairs[2 * lo] = last;
+                a.pairs[2 * lo + 1] = static_cast<int>(p);
+                row[has - 1] = static_cast<int>(p);
+                atomicAdd(a.new_refcount + last, -1);
+            } else {
+                row[has + nth - ((need & kCopies) != 0 ? 1 : 0)] = static_cast<int>(p);
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(kTableWaves *kWave) void page_table_rows(UpdateArgs a) { lay_aside<kTableWaves>(a, Crew{blockIdx.x, gridDim.x}); }
+__global__ __launch_bounds__(kTableWaves *kWave) void page_table_count(UpdateArgs a) { count_rows<kTableWaves>(a, Crew{blockIdx.x, gridDim.x}); }
+__global__ __launch_bounds__(kTableWaves *kWave) void page_table_needs(UpdateArgs a) {
+    __shared__ uint32_t slots[kTableWaves];
+    work_out<kTableWaves>(a, Crew{blockIdx.x, gridDim.x}, slots);
+}
+__global__ __launch_bounds__(kTableWaves *kWave) void page_table_fresh(UpdateArgs a) {
+    __shared__ uint32_t ends[kMostTableRows];
+    __shared__ uint64_t slots[kTableWaves];
+    hand_out<kTableWaves>(a, Crew{blockIdx.x, gridDim.x}, ends, slots);
+}
+__global__ __launch_bounds__(kOneWaves *kWave) void page_table_update_one(UpdateArgs a) {
+    __shared__ uint32_t ends[kMostTableRows];
+    __shared__ uint64_t slots[kOneWaves];
+    const Crew alone{0, 1};
+    lay_aside<kOneWaves>(a, alone);
+    phase_end();
+    count_rows<kOneWaves>(a, alone);
+    phase_end();
+    work_out<kOneWaves>(a, alone, reinterpret_cast<uint32_t *>(slots));
+    phase_end();
+    hand_out<kOneWaves>(a, alone, ends, slots);
+}
+
+}// namespace
+
+infiniopStatus_t amdPageTableUpdate(PageTableUpdateAmdDescriptor_t desc, void *workspace, uint64_t workspace_size, void *new_table, void *new_lengths,
+                                    void *new_refcount, void *pairs, void *result, void const *table, void const *lengths, void const *refcount,
+                                    void const *source, void const *grow, void *stream) {
+    const PageTableUpdateAmdDescriptor &d = *desc;
+    const amd::TableSizes &z = d.sizes;
+    if (z.old_rows.rows == 0) {
+        return STATUS_SUCCESS;
+    }
+    if (workspace == nullptr || workspace_size < d.workspace) {
+        return STATUS_MEMORY_NOT_ALLOCATED;
+    }
+    for (const void *p : {static_cast<const void *>(new_table), static_cast<const void *>(new_lengths), static_cast<const void *>(new_refcount),
+                          static_cast<const void *>(pairs), static_cast<const void *>(result), table, lengths, refcount, source, grow}) {
+        if (p == nullptr) return STATUS_BAD_PARAM;
+    }
+    if (reinterpret_cast<uintptr_t>(workspace) % 8 != 0 || (new_table == table && z.new_rows.stride != z.old_rows.stride)) {
+        return STATUS_BAD_PARAM;
+    }
+    AMD_CHECK_HIP(hipSetDevice(d.device_id), STATUS_BAD_DEVICE);
+    const uint64_t chunks = amd::chunks_of(z.pages), rows = z.old_rows.rows;
+    auto *words = static_cast<uint64_t *>(workspace);
+    auto *counts = reinterpret_cast<uint32_t *>(words + chunks * kChunkWords);
+    const UpdateArgs a{static_cast<const int *>(table), static_cast<const int *>(lengths), static_cast<const int *>(refcount),
+                       static_cast<const int *>(source), static_cast<const int *>(grow), static_cast<int *>(new_table),
+                       static_cast<int *>(new_lengths), static_cast<int *>(new_refcount), static_cast<int *>(pairs), static_cast<int *>(result),
+                       z.old_rows.stride, z.new_rows.stride, z.old_rows.rows, z.old_rows.cols, z.pages, z.page, amd::fast_div(z.page),
+                       words, counts, counts + chunks, counts + chunks + rows, reinterpret_cast<int *>(counts + chunks + 2 * rows)};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (rows * z.old_rows.cols + z.pages <= 16384) {
+        page_table_update_one<<<1, kOneWaves * amd::kWave, 0, s>>>(a);
+    } else {
+        const unsigned by_row = static_cast<unsigned>(rows < 1024 ? rows : 1024), by_chunk = static_cast<unsigned>(chunks < 1024 ? chunks : 1024);
+        page_table_rows<<<by_row, kTableWaves * amd::kWave, 0, s>>>(a);
+        page_table_count<<<by_row, kTableWaves * amd::kWave, 0, s>>>(a);
+        page_table_needs<<<by_row > by_chunk ? by_row : by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
+        page_table_fresh<<<by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
+    }
+    AMD_CHECK_HIP(hipGetLastError(), STATUS_EXECUTION_FAILED);
+    return STATUS_SUCCESS;
+}

@@ -1,0 +1,41 @@
+// amd-gpu back end of PagedAttention.
+#ifndef INFINIOP_AMD_PAGED_ATTENTION_H
+#define INFINIOP_AMD_PAGED_ATTENTION_H
+
+#include "../../paged_cache.h"
+
+// How a call's work is cut up.  A tile is up to `tile_rows` query rows (token by
+// head of one K/V head's group) of one sequence; a unit is a tile over a range of
+// keys, and what one workgroup computes.  `target` units of a K/V head are aimed
+// at; a tile is split over several units where that gives fewer.
+struct PagedAttentionShape {
+    uint32_t tile_rows;
+    uint32_t most_tiles;// of one K/V head, whatever the offsets
+    uint32_t target;
+};
+
+struct PagedAttentionAmdDescriptor {
+    Device device;
+    int device_id;
+    bool bf16;// q and out, else F16
+    amd::PagedCache cache;
+    amd::PagedRows rows;
+    uint32_t tokens, group, max_tokens;
+    int64_t q_token, q_head, out_token, out_head;// elements
+    float scale;
+    PagedAttentionShape shape;
+    uint64_t workspace;
+};
+typedef PagedAttentionAmdDescriptor *PagedAttentionAmdDescriptor_t;
+
+infiniopStatus_t amdCreatePagedAttentionDescriptor(AmdHandle_t handle, PagedAttentionAmdDescriptor_t *desc_ptr, infiniopTensorDescriptor_t out,
+                                                   infiniopTensorDescriptor_t q, infiniopTensorDescriptor_t k_cache, infiniopTensorDescriptor_t v_cache,
+                                                   infiniopTensorDescriptor_t k_scale, infiniopTensorDescriptor_t v_scale,
+                                                   infiniopTensorDescriptor_t table, infiniopTensorDescriptor_t offsets,
+                                                   infiniopTensorDescriptor_t lengths, uint64_t max_tokens, float scale);
+infiniopStatus_t amdPagedAttention(PagedAttentionAmdDescriptor_t desc, void *workspace, uint64_t workspace_size, void *out, void const *q,
+                                   void const *k_cache, void const *v_cache, void const *k_scale, void const *v_scale, void const *table,
+                                   void const *offsets, void const *lengths, void *stream);
+infiniopStatus_t amdDestroyPagedAttentionDescriptor(PagedAttentionAmdDescriptor_t desc);
+
+#endif

@@ -1,0 +1,529 @@
+// gfx950 PagedAttention for few query rows: decoding.
+//     S = K q^T,  P = exp2(scale S - m),  O = V^T P^T      all transposed, keys down the accumulator's rows
+// A wavefront takes 32 keys at a time, straight from the cache to registers, and up
+// to 16 query rows (NT times) that share them.  Two v_mfma_f32_16x16x32 outputs hold
+// 8 keys of one query in every lane, and those very 8 numbers, rounded to fp16, are
+// that lane's share of the second product's operand: the matrix unit's k index is a
+// label that both operands only have to agree on, so nothing of P is exchanged
+// between lanes.  For V a lane holds the same 8 keys of dim / 16 neighbouring
+// columns: byte permutations turn 8 keys x 4 columns round in registers.
+// Codes are exact in fp16; q is multiplied by a power of two for each row that
+// brings its largest element to [1, 2), so that it is too (but for what is 2^24 times
+// smaller than that element), whatever its type.  Scores, maxima, sums and O are fp32.
+// P in fp16 costs each weight at most 2^-11 of itself, as much as rounding `out` to
+// fp16 does and an eighth of bf16; the scale of a V block goes into P, relative to
+// the largest one so far.  P is lifted by 2^10, so that of a weight too small for
+// that at most 2^-35 of the largest is lost, and the sum of very many small weights
+// beside a large one is kept: m is the maximum less 10.
+// The maximum is moved only when a score exceeds it by 2^4, and the V scale when one
+// is over twice as large (P stays below 2^15), which leaves the usual step without an
+// exchange between lanes.
+// Bound by reading K and V once from HBM.
+#include "paged_attention_units.h"
+
+namespace {
+
+using namespace amd;
+
+constexpr int kWaves = 4;
+constexpr float kLift = 10.0f;   // log2 of P where the score is the running maximum
+constexpr float kSlack = 4.0f;   // log2 by which a score may exceed the running maximum
+constexpr float kNone = -1.0e30f;// the maximum of no score
+
+// maximum and sum over the four lanes that hold one query row
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// What a lane reads of 32 keys: of K, 16 bytes of each 64 columns of keys (lane % 16) of either half; of V,
+// BYTES neighbouring columns of keys 4 (lane / 16) .. + 3 of either half.
+template<int DP>
+struct Tile {
+    static constexpr int kChunks = DP / 64, kWords = DP / 64;
+    u32x4 k[2][kChunks];
+    uint32_t v[2][4][kWords];
+};
+
+template<int WORDS>
+__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[WORDS]) {
+    if constexpr (WORDS == 1) {
+        w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p));
+    } else if constexpr (WORDS == 2) {
+        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p));
+        w[0] = x.x;
+        w[1] = x.y;
+    } else if constexpr (WORDS == 3) {// at 4-byte boundaries
+        typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+        typedef u32x3 __attribute__((aligned(4))) u32x3_any;
+        const u32x3 x = __builtin_nontemporal_load(reinterpret_cast<const u32x3_any *>(p));
+        w[0] = x.x;
+        w[1] = x.y;
+        w[2] = x.z;
+    } else {
+        const u32x4 x = ld16_stream(p);
+        w[0] = x.x;
+        w[1] = x.y;
+        w[2] = x.z;
+        w[3] = x.w;
+    }
+}
+
+template<bool FP8, int DP, int NT>
+__global__ __launch_bounds__(kWaves *kWave) void paged_attention_rows(AttentionArgs a) {
+    constexpr int KS = DP / 32, CH = DP / 64, VB = DP / 16, WORDS = DP / 64;
+    __shared__ uint64_t slots[kWaves];
+    __shared__ Unit shared_unit;
+    __shared__ float stat[2][kWaves][16 * NT];
+    __shared__ f32x4 meet[2][NT * VB][kWave];
+    Unit u;
+    const uint32_t head = blockIdx.x % a.kv_heads;
+    if (!find_unit<kWaves, false>(a, blockIdx.x / a.kv_heads, slots, &shared_unit, &u)) return;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave)));
+    const uint32_t n16 = lane & 15u, g = lane >> 4;
+    const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens;
+    const uint32_t row0 = u.tile * a.tile_rows, rows = tokens * a.group;
+    // token i sees the places below seen + i + 1
+    const int seen = static_cast<int>(u.length) - static_cast<int>(u.count);
+    const auto sees = [&](uint32_t token) { return static_cast<uint32_t>(seen + static_cast<int>(token) < 0 ? 0 : seen + static_cast<int>(token) + 1); };
+    const uint32_t row_end = row0 + a.tile_rows < rows ? row0 + a.tile_rows : rows;
+    const uint32_t all_see = sees(fast_quotient(row0, a.by_group)), some_see = sees(fast_quotient(row_end - 1, a.by_group));
+
+    // the query rows, as the second operand of S: lane's row, 8 columns of each step of 32
+    f16x8 q[NT][KS];
+    float factor[NT];
+    uint32_t limit[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const uint32_t r = row0 + t * 16 + n16, token = fast_quotient(r, a.by_group);
+        const bool mine = r < row_end;
+        limit[t] = mine ? sees(token) : 0;
+        float x[KS][8];
+        float top = 0.0f;
+        const uint16_t *p = a.q + static_cast<int64_t>(u.first + token) * a.q_token + static_cast<int64_t>(head * a.group + (r - token * a.group)) * a.q_head;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const uint32_t d = c * 64 + g * 16;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u32x4 w = {0, 0, 0, 0};
+                if (mine && d < a.dim) w = ld16_any(p + d + h * 8);
+                float y[8];
+                if (a.bf16) widen8<BF16Rne>(w, y);
+                else widen8<F16Ref>(w, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[2 * c + h][i] = y[i];
+                    top = fmaxf(top, fabsf(y[i]));
+                }
+            }
+        }
+        top = quad_max(top);
+        const int e = top > 0.0f ? static_cast<int>(__float_as_uint(top) >> 23) - 127 : 0;
+        factor[t] = ldexpf(a.scale, e);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[t][s][i] = static_cast<_Float16>(ldexpf(x[s][i], -e));
+        }
+    }
+
+    f32x4 o[NT][VB];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = kNone;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VB; ++j) o[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float v_top = 0.0f, v_inv = 0.0f;// the largest V scale that O stands relative to, and its inverse
+
+    // the lane's places within a page, relative to the half's first key
+    uint32_t k_off[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) k_off[c] = n16 * a.k_at.token + (c * 64 + g * 16 < a.dim ? c * 64 + g * 16 : 0);// (q is 0 behind dim)
+    const uint32_t v_off = g * 4 * a.v_at.token + (n16 * VB < a.dim ? n16 * VB : 0);                             // (not stored behind dim)
+    const uint8_t *k_base = a.k + static_cast<uint64_t>(head) * a.k_at.head, *v_base = a.v + static_cast<uint64_t>(head) * a.v_at.head;
+    const float *ks_base = a.k_scale + static_cast<int64_t>(head) * a.k_at.s_head, *vs_base = a.v_scale + static_cast<int64_t>(head) * a.v_at.s_head;
+    const int *table = a.rows.table + u.row * a.rows.stride;
+
+    const uint32_t end = (some_see + kStepKeys - 1) / kStepKeys;
+    const uint32_t s0 = u.chunk * u.steps, s1 = s0 + u.steps < end ? s0 + u.steps : end;
+    // steps s0 + wave, + 4, ...: page, place in it and scales of 32 of them are read at once, a half step by each lane
+    for (uint32_t base = s0 + wave; base < s1; base += kWaves * 32) {
+        int page = -1;
+        uint32_t place = 0;
+        float k_scale = 0.0f, v_scale = 0.0f;
+        {
+            const uint32_t key = ((base + kWaves * (lane >> 1)) * 2 + (lane & 1)) * 16;
+            if (key < u.length) {
+                const uint32_t col = fast_quotient(key, a.rows.by_page);
+                page = table[col];
+                place = key - col * a.rows.page;
+                if (static_cast<uint32_t>(page) < a.pages) {
+                    const uint32_t block = fast_quotient(place, a.by_block);
+                    k_scale = ks_base[page * a.k_at.s_page + block];
+                    v_scale = vs_base[page * a.v_at.s_page + block];
+                } else {
+                    page = -1;
+                }
+            }
+        }
+        const uint32_t count = (s1 - base + kWaves - 1) / kWaves < 32 ? (s1 - base + kWaves - 1) / kWaves : 32;
+        const auto load = [&](uint32_t i, Tile<DP> &t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int pg = __builtin_amdgcn_readlane(page, 2 * i + h);
+                const uint32_t at = __builtin_amdgcn_readlane(place, 2 * i + h);
+                const int64_t there = pg < 0 ? 0 : pg;// (no page: any place will do, the keys are masked)
+                const uint8_t *kp = k_base + there * a.k_at.page + static_cast<uint64_t>(at) * a.k_at.token;
+                const uint8_t *vp = v_base + there * a.v_at.page + static_cast<uint64_t>(at) * a.v_at.token;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) t.k[h][c] = ld16_stream(kp + k_off[c]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) load_words<WORDS>(vp + static_cast<uint64_t>(j) * a.v_at.token + v_off, t.v[h][j]);
+            }
+        };
+        const auto step = [&](uint32_t i, Tile<DP> &t) {
+            const uint32_t key0 = (base + kWaves * i) * kStepKeys;
+            const int pg0 = __builtin_amdgcn_readlane(page, 2 * i), pg1 = __builtin_amdgcn_readlane(page, 2 * i + 1);
+            const float ks[2] = {__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, k_scale), 2 * i)),
+                                 __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, k_scale), 2 * i + 1))};
+            const float vs[2] = {__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v_scale), 2 * i)),
+                                 __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v_scale), 2 * i + 1))};
+            f32x4 s[NT][2];
+#pragma unroll
+            for (int t2 = 0; t2 < NT; ++t2) s[t2][0] = s[t2][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int e = 0; e < KS; ++e) {
+                    const uint32_t w0 = prepare_codes<FP8>(t.k[h][e / 2][e % 2 * 2]), w1 = prepare_codes<FP8>(t.k[h][e / 2][e % 2 * 2 + 1]);
+                    f16x8 x;
+                    const f16x2 p0 = pair_of<FP8, false>(w0), p1 = pair_of<FP8, true>(w0), p2 = pair_of<FP8, false>(w1), p3 = pair_of<FP8, true>(w1);
+                    x = f16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+#pragma unroll
+                    for (int t2 = 0; t2 < NT; ++t2) s[t2][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[t2][e], s[t2][h], 0, 0, 0);
+                }
+            }
+            const bool masked = pg0 < 0 || pg1 < 0 || key0 + kStepKeys > all_see;
+            if (masked) {// also V's codes behind the row's end, which may be anything
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (key0 + h * 16 + g * 4 + j >= u.length || (h == 0 ? pg0 : pg1) < 0) {
+#pragma unroll
+                            for (int w = 0; w < WORDS; ++w) t.v[h][j][w] = 0;
+                        }
+                    }
+                }
+            }
+            const float v_now = fmaxf(vs[0], vs[1]);
+            if (v_now > 2.0f * v_top) {
+                // (never below 2^-100, whose inverse is far from infinity)
+                const float next = fmaxf(v_now, 0x1p-100f), by = v_top / next;
+                v_top = next;
+                v_inv = 1.0f / next;
+#pragma unroll
+                for (int t2 = 0; t2 < NT; ++t2) {
+#pragma unroll
+                    for (int j = 0; j < VB; ++j) o[t2][j] *= by;
+                }
+            }
+            f16x8 p[NT];
+#pragma unroll
+            for (int t2 = 0; t2 < NT; ++t2) {
+                float x[8];
+                const float f0 = factor[t2] * ks[0], f1 = factor[t2] * ks[1];
+#pragma unroll
+                for (int i2 = 0; i2 < 4; ++i2) {
+                    x[i2] = s[t2][0][i2] * f0;
+                    x[4 + i2] = s[t2][1][i2] * f1;
+                }
+                if (masked) {
+#pragma unroll
+                    for (int i2 = 0; i2 < 8; ++i2) {
+                        const bool gone = key0 + (i2 / 4) * 16 + g * 4 + i2 % 4 >= limit[t2] || (i2 < 4 ? pg0 : pg1) < 0;
+                        x[i2] = gone ? -__builtin_inff() : x[i2];
+                    }
+                }
+                float high = x[0];
+#pragma unroll
+                for (int i2 = 1; i2 < 8; ++i2) high = fmaxf(high, x[i2]);
+                if (__builtin_amdgcn_ballot_w64(high > m[t2] + (kLift + kSlack)) != 0) {
+                    const float next = fmaxf(m[t2], quad_max(high) - kLift), by = __builtin_amdgcn_exp2f(m[t2] - next);
+                    m[t2] = next;
+                    l[t2] *= by;
+#pragma unroll
+                    for (int j = 0; j < VB; ++j) o[t2][j] *= by;
+                }
+                float sum = 0.0f;
+                const float r0 = vs[0] * v_inv, r1 = vs[1] * v_inv;
+                float y[8];
+#pragma unroll
+                for (int i2 = 0; i2 < 8; ++i2) {
+                    y[i2] = __builtin_amdgcn_exp2f(x[i2] - m[t2]);
+                    sum += y[i2];
+                    y[i2] *= i2 < 4 ? r0 : r1;
+                }
+                l[t2] += sum;
+#pragma unroll
+                for (int i2 = 0; i2 < 8; i2 += 2) {
+                    const f16x2 w = __builtin_convertvector((f32x2{y[i2], y[i2 + 1]}), f16x2);
+                    p[t2][i2] = w.x;
+                    p[t2][i2 + 1] = w.y;
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+                uint32_t x[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[h][j] = prepare_codes<FP8>(t.v[h][j][w]);
+                }
+                // columns 0 and 1 (2 and 3) of keys 0, 1 and of keys 2, 3
+                uint32_t pair[2][2][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        pair[h][j][0] = __builtin_amdgcn_perm(x[h][2 * j + 1], x[h][2 * j], 0x05010400u);
+                        pair[h][j][1] = __builtin_amdgcn_perm(x[h][2 * j + 1], x[h][2 * j], 0x07030602u);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const auto two = [&](int h, int j) { return c % 2 ? pair_of<FP8, true>(pair[h][j][c / 2]) : pair_of<FP8, false>(pair[h][j][c / 2]); };
+                    const f16x2 y0 = two(0, 0), y1 = two(0, 1), y2 = two(1, 0), y3 = two(1, 1);
+                    const f16x8 y = {y0.x, y0.y, y1.x, y1.y, y2.x, y2.y, y3.x, y3.y};
+#pragma unroll
+                    for (int t2 = 0; t2 < NT; ++t2) o[t2][w * 4 + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, p[t2], o[t2][w * 4 + c], 0, 0, 0);
+                }
+            }
+        };
+        Tile<DP> even, odd;
+        load(0, even);
+        for (uint32_t i = 0; i < count; i += 2) {
+            if (i + 1 < count) load(i + 1, odd);
+            step(i, even);
+            if (i + 1 < count) {
+                if (i + 2 < count) load(i + 2, even);
+                step(i + 1, odd);
+            }
+        }
+    }
+
+    // the four wavefronts' sums, to the first: maxima, then O by halves
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        l[t] = quad_sum(l[t]);
+        if (g == 0) {
+            stat[0][wave][t * 16 + n16] = m[t];
+            stat[1][wave][t * 16 + n16] = l[t];
+        }
+    }
+    __syncthreads();
+    float total[NT], high[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        high[t] = kNone;
+        total[t] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) high[t] = fmaxf(high[t], stat[0][w][t * 16 + n16]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) total[t] += stat[1][w][t * 16 + n16] * __builtin_amdgcn_exp2f(stat[0][w][t * 16 + n16] - high[t]);
+        const float by = v_top * __builtin_amdgcn_exp2f(m[t] - high[t]);
+#pragma unroll
+        for (int j = 0; j < VB; ++j) o[t][j] *= by;
+    }
+    if (wave >= 2) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int j = 0; j < VB; ++j) meet[wave - 2][t * VB + j][lane] = o[t][j];
+        }
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int j = 0; j < VB; ++j) o[t][j] += meet[wave][t * VB + j][lane];
+        }
+    }
+    if (wave == 1) {// (its own half of the room: only it has read that)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int j = 0; j < VB; ++j) meet[1][t * VB + j][lane] = o[t][j];
+        }
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int j = 0; j < VB; ++j) o[t][j] += meet[1][t * VB + j][lane];
+        const uint32_t r = row0 + t * 16 + n16;
+        if (r >= row_end) continue;
+        // o[t][j][i] is column (4 g + i) VB + j of the row
+        if (u.chunks > 1) {
+            const uint64_t at = (static_cast<uint64_t>(u.slot + u.chunk) * a.kv_heads + head) * a.tile_rows + t * 16 + n16;
+            if (g == 0) {
+                a.part_stat[2 * at] = high[t];
+                a.part_stat[2 * at + 1] = total[t];
+            }
+            if (total[t] == 0.0f) continue;// not read
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int j = 0; j < VB; j += 4) {
+                    *reinterpret_cast<f32x4 *>(a.part_out + at * DP + (4 * g + i) * VB + j) = f32x4{o[t][j][i], o[t][j + 1][i], o[t][j + 2][i], o[t][j + 3][i]};
+                }
+            }
+        } else {
+            const float by = total[t] > 0.0f ? 1.0f / total[t] : 0.0f;
+            const uint32_t token = fast_quotient(r, a.by_group);
+            uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + static_cast<int64_t>(head * a.group + (r - token * a.group)) * a.out_head;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t d = (4 * g + i) * VB;
+                if (d >= a.dim) continue;
+#pragma unroll
+                for (int j = 0; j < VB; j += 4) {
+                    *reinterpret_cast<u32x2_any *>(p + d + j) = u32x2{narrow2_rne(a.bf16, o[t][j][i] * by, o[t][j + 1][i] * by),
+                                                                      narrow2_rne(a.bf16, o[t][j + 2][i] * by, o[t][j + 3][i] * by)};
+                }
+            }
+        }
+    }
+}
+
+// The units of a tile together: a wavefront takes one query row.
+template<int DP>
+__global__ __launch_bounds__(kWaves *kWave) void paged_attention_join(AttentionArgs a) {
+    constexpr int PER = DP / 64;
+    __shared__ uint64_t slots[kWaves];
+    __shared__ Unit shared_unit;
+    Unit u;
+    const uint32_t head = blockIdx.x % a.kv_heads;
+    if (!find_unit<kWaves, true>(a, blockIdx.x / a.kv_heads, slots, &shared_unit, &u)) return;
+    const uint32_t lane = threadIdx.x & (kWave - 1), in_tile = blockIdx.y * kWaves + threadIdx.x / kWave;
+    const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens;
+    const uint32_t r = u.tile * a.tile_rows + in_tile;
+    if (r >= tokens * a.group) return;
+    const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * a.tile_rows + in_tile; };
+    float high = kNone;
+    for (uint32_t c = lane; c < u.chunks; c += kWave) high = fmaxf(high, a.part_stat[2 * at(c)]);
+    high = wave_max(high);
+    float total = 0.0f, o[PER] = {};
+    for (uint32_t base = 0; base < u.chunks; base += kWave) {
+        const uint32_t mine = base + lane;
+        float by = 0.0f, l = 0.0f;
+        if (mine < u.chunks) {
+            l = a.part_stat[2 * at(mine) + 1];
+            by = l > 0.0f ? __builtin_amdgcn_exp2f(a.part_stat[2 * at(mine)] - high) : 0.0f;
+        }
+        total += wave_sum(l * by);
+        const uint32_t n = u.chunks - base < kWave ? u.chunks - base : kWave;
+        for (uint32_t c = 0; c < n; ++c) {
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, by), c));
+            if (w == 0.0f) continue;// (a unit that saw nothing has written nothing)
+            const float *p = a.part_out + at(base + c) * DP + lane * PER;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) o[i] += w * p[i];
+        }
+    }
+    const float by = total > 0.0f ? 1.0f / total : 0.0f;
+    const uint32_t token = fast_quotient(r, a.by_group);
+    uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + static_cast<int64_t>(head * a.group + (r - token * a.group)) * a.out_head;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (lane * PER + i < a.dim) p[lane * PER + i] = static_cast<uint16_t>(narrow2_rne(a.bf16, o[i] * by, 0.0f));
+    }
+}
+
+template<bool FP8, int DP>
+void launch(const PagedAttentionAmdDescriptor &d, const AttentionArgs &a, hipStream_t s) {
+    const unsigned units = (d.shape.target + d.shape.most_tiles) * d.cache.kv_heads;
+    if constexpr (DP <= 128) {
+        if (d.shape.tile_rows == 16) paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
+        else paged_attention_rows<FP8, DP, 2><<<units, kWaves * kWave, 0, s>>>(a);
+    } else {
+        paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
+    }
+    // a tile of several units has two at least
+    paged_attention_join<DP><<<dim3(d.shape.target * d.cache.kv_heads, d.shape.tile_rows / kWaves), kWaves * kWave, 0, s>>>(a);
+}
+
+template<bool FP8>
+void launch(const PagedAttentionAmdDescriptor &d, const AttentionArgs &a, hipStream_t s) {
+    if (d.cache.dim <= 64) launch<FP8, 64>(d, a, s);
+    else if (d.cache.dim <= 128) launch<FP8, 128>(d, a, s);
+    else if (d.cache.dim <= 192 && d.cache.dim % 48 == 0) launch<FP8, 192>(d, a, s);// (12 columns a lane: whole lanes)
+    else launch<FP8, 256>(d, a, s);
+}
+
+}// namespace
+
+infiniopStatus_t amdPagedAttention(PagedAttentionAmdDescriptor_t desc, void *workspace, uint64_t workspace_size, void *out, void const *q,
+                                   void const *k_cache, void const *v_cache, void const *k_scale, void const *v_scale, void const *table,
+                                   void const *offsets, void const *lengths, void *stream) {
+    const PagedAttentionAmdDescriptor &d = *desc;
+    if (d.tokens == 0 || d.rows.rows == 0) {
+        return STATUS_SUCCESS;
+    }
+    if (workspace == nullptr || workspace_size < d.workspace) {
+        return STATUS_MEMORY_NOT_ALLOCATED;
+    }
+    for (const void *p : {static_cast<const void *>(out), q, k_cache, v_cache, k_scale, v_scale, table, offsets, lengths}) {
+        if (p == nullptr) return STATUS_BAD_PARAM;
+    }
+    if (!amd::aligned16(k_cache) || !amd::aligned16(v_cache) || !amd::aligned16(workspace)) {
+        return STATUS_BAD_PARAM;
+    }
+    AMD_CHECK_HIP(hipSetDevice(d.device_id), STATUS_BAD_DEVICE);
+    const uint64_t slots = 2ull * d.shape.target * d.cache.kv_heads * d.shape.tile_rows;
+    auto *parts = static_cast<float *>(workspace);
+    const AttentionArgs a{
+        {static_cast<const int *>(table), static_cast<const int *>(offsets), static_cast<const int *>(lengths), d.rows.stride, d.rows.rows, d.rows.cols,
+         d.tokens, d.cache.page, amd::fast_div(d.cache.page)},
+        static_cast<const uint8_t *>(k_cache),
+        static_cast<const uint8_t *>(v_cache),
+        static_cast<const float *>(k_scale),
+        static_cast<const float *>(v_scale),
+        d.cache.k,
+        d.cache.v,
+        static_cast<const uint16_t *>(q),
+        static_cast<uint16_t *>(out),
+        d.q_token,
+        d.q_head,
+        d.out_token,
+        d.out_head,
+        d.cache.pages,
+        d.cache.kv_heads,
+        d.cache.dim,
+        d.group,
+        d.max_tokens,
+        d.shape.tile_rows,
+        amd::fast_div(d.group),
+        amd::fast_div(d.cache.block),
+        amd::fast_div(d.shape.tile_rows),
+        d.scale * 1.44269504088896340736f,
+        1.0f / static_cast<float>(d.shape.target),
+        8,
+        d.bf16,
+        parts + 2 * slots,
+        parts};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    d.cache.fp8 ? launch<true>(d, a, s) : launch<false>(d, a, s);
+    AMD_CHECK_HIP(hipGetLastError(), STATUS_EXECUTION_FAILED);
+    return STATUS_SUCCESS;
+}

@@ -1,0 +1,92 @@
+// Device-side pieces that the kernels of the paged cache share: the rows of a
+// ragged batch, whole-number sums and scans over a workgroup, and 8-bit codes as
+// fp16 pairs.  Include from .hip files only.
+#ifndef INFINIOP_AMD_PAGED_KERNEL_H
+#define INFINIOP_AMD_PAGED_KERNEL_H
+
+#include "../devices/amd/kernel_amd.h"
+#include "paged_cache.h"
+
+namespace amd {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 __attribute__((aligned(2))) u32x2_any;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// ---- the rows of a batch ----------------------------------------------------
+struct RaggedRows {
+    const int *table;// [rows, cols]
+    const int *offsets, *lengths;
+    int64_t stride;// of the table
+    uint32_t rows, cols, tokens, page;
+    FastDiv by_page;
+};
+
+// Row r's new tokens [first, first + count) of the call and its length with
+// them, brought into range whatever the arrays hold: tokens within the call's,
+// a length within the table.
+struct RowSpan {
+    uint32_t first, count, length;
+};
+__device__ __forceinline__ RowSpan row_span(const RaggedRows &b, uint32_t r) {
+    const int tokens = static_cast<int>(b.tokens), room = static_cast<int>(b.cols * b.page);// < 2^31
+    const int from = b.offsets[r], to = b.offsets[r + 1], len = b.lengths[r];
+    const int lo = from < 0 ? 0 : from > tokens ? tokens : from, hi = to < lo ? lo : to > tokens ? tokens : to;
+    return RowSpan{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi - lo), static_cast<uint32_t>(len < 0 ? 0 : len > room ? room : len)};
+}
+
+// ---- whole-number sums over a workgroup of WAVES wavefronts --------------------
+// slots: LDS, WAVES values; one use of it has to end with a barrier before the next begins.
+__device__ __forceinline__ uint64_t shuffle_up64(uint64_t v, int by) {
+    const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), by), hi = __shfl_up(static_cast<uint32_t>(v >> 32), by);
+    return lo | static_cast<uint64_t>(hi) << 32;
+}
+// The sum of the lower lanes' values (exclusive), and of all in `total`.
+template<int WAVES>
+__device__ __forceinline__ uint64_t block_scan64(uint64_t v, uint64_t *slots, uint64_t *total) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    uint64_t sum = v;
+#pragma unroll
+    for (int by = 1; by < kWave; by *= 2) {
+        const uint64_t other = shuffle_up64(sum, by);
+        if (lane >= by) sum += other;
+    }
+    if (lane == kWave - 1) slots[wave] = sum;
+    __syncthreads();
+    uint64_t before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+        if (i < wave) before += slots[i];
+        all += slots[i];
+    }
+    __syncthreads();
+    *total = all;
+    return before + sum - v;
+}
+
+// ---- codes as fp16 ------------------------------------------------------------
+// Both types are exact in fp16: whole numbers up to 128, and e4m3.
+// An int8 with its sign bit turned over, as the low byte of 0x64xx, is the fp16
+// number 1024 + 128 + value; one packed subtraction leaves the value.
+__device__ __forceinline__ f16x2 bias_off(uint32_t pair) {
+    return __builtin_bit_cast(f16x2, pair) + f16x2{static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+}
+// int8 codes come with their sign bits turned over (prepare_codes)
+template<bool FP8>
+__device__ __forceinline__ uint32_t prepare_codes(uint32_t w) {
+    return FP8 ? w : w ^ 0x80808080u;
+}
+// bytes 2 * HI and 2 * HI + 1 of a word
+template<bool FP8, bool HI>
+__device__ __forceinline__ f16x2 pair_of(uint32_t w) {
+    if constexpr (FP8) {
+        return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI);
+    } else {
+        return bias_off(__builtin_amdgcn_perm(0x64646464u, w, HI ? 0x04030402u : 0x04010400u));
+    }
+}
+
+}// namespace amd
+
+#endif

@@ -42,6 +42,7 @@ _TABLE = {
     "BF16": (1, 1, 2, 7, 8),
     "F32": (1, 1, 4, 23, 8),
     "F64": (1, 1, 8, 52, 11),
+    "F8E4M3": (1, 1, 1, 3, 4),
 }
 _NAMES = {v: k for k, v in _TABLE.items()}
 
@@ -57,5 +58,6 @@ F16 = DataLayout(*_TABLE["F16"])
 BF16 = DataLayout(*_TABLE["BF16"])
 F32 = DataLayout(*_TABLE["F32"])
 F64 = DataLayout(*_TABLE["F64"])
+F8E4M3 = DataLayout(*_TABLE["F8E4M3"])  # include/infiniop_paged.h
 
 __all__ = ["DataLayout"] + list(_TABLE)

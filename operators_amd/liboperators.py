@@ -1,4 +1,6 @@
-"""Loader and ctypes prototypes for libinfiniop.so (amd-gpu build).
+"""Loader and ctypes prototypes for libinfiniop.so (amd-gpu build), and for
+libinfiniop_paged.so beside it: the operators of the paged cache
+(include/infiniop_paged.h), which the reference does not have.
 
 Counterpart of the reference's operatorspy/liboperators.py:11-73: the library is
 looked up under $INFINI_ROOT/lib when INFINI_ROOT is set, otherwise in this
@@ -14,6 +16,7 @@ from .data_layout import DataLayout
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libinfiniop.so"
+PAGED_LIB_NAME = "libinfiniop_paged.so"
 
 
 class TensorDescriptor(Structure):
@@ -85,6 +88,26 @@ class RandomSampleDescriptor(_OpDescriptor):
     pass
 
 
+class KVCacheAppendDescriptor(_OpDescriptor):
+    pass
+
+
+class PagedAttentionDescriptor(_OpDescriptor):
+    pass
+
+
+class KVCacheCopyDescriptor(_OpDescriptor):
+    pass
+
+
+class PageTableUpdateDescriptor(_OpDescriptor):
+    pass
+
+
+class PageTableCompactDescriptor(_OpDescriptor):
+    pass
+
+
 infiniopAddDescriptor_t = POINTER(AddDescriptor)
 infiniopRMSNormDescriptor_t = POINTER(RMSNormDescriptor)
 infiniopRoPEDescriptor_t = POINTER(RoPEDescriptor)
@@ -96,6 +119,11 @@ infiniopMatmulDescriptor_t = POINTER(MatmulDescriptor)
 infiniopMLPDescriptor_t = POINTER(MLPDescriptor)
 infiniopAttentionDescriptor_t = POINTER(AttentionDescriptor)
 infiniopRandomSampleDescriptor_t = POINTER(RandomSampleDescriptor)
+infiniopKVCacheAppendDescriptor_t = POINTER(KVCacheAppendDescriptor)
+infiniopPagedAttentionDescriptor_t = POINTER(PagedAttentionDescriptor)
+infiniopKVCacheCopyDescriptor_t = POINTER(KVCacheCopyDescriptor)
+infiniopPageTableUpdateDescriptor_t = POINTER(PageTableUpdateDescriptor)
+infiniopPageTableCompactDescriptor_t = POINTER(PageTableCompactDescriptor)
 
 
 class CTensor:
@@ -106,11 +134,11 @@ class CTensor:
         self.data = data
 
 
-def library_path():
+def library_path(name=LIB_NAME):
     root = os.environ.get("INFINI_ROOT")
     if root:
-        return os.path.join(root, "lib", LIB_NAME)
-    return os.path.join(_PKG_DIR, "lib", LIB_NAME)
+        return os.path.join(root, "lib", name)
+    return os.path.join(_PKG_DIR, "lib", name)
 
 
 # name -> (argtypes); every entry point returns an infiniopStatus_t (int32)
@@ -166,6 +194,34 @@ _PROTOTYPES = {
 
 EXPORTED_SYMBOLS = tuple(_PROTOTYPES)
 
+# the same for libinfiniop_paged.so
+_PAGED_PROTOTYPES = {
+    "infiniopCreateKVCacheAppendDescriptor": [infiniopHandle_t, POINTER(infiniopKVCacheAppendDescriptor_t)] + [infiniopTensorDescriptor_t] * 9,
+    "infiniopGetKVCacheAppendWorkspaceSize": [infiniopKVCacheAppendDescriptor_t, POINTER(c_uint64)],
+    "infiniopKVCacheAppend": [infiniopKVCacheAppendDescriptor_t, c_void_p, c_uint64] + [c_void_p] * 10,
+    "infiniopDestroyKVCacheAppendDescriptor": [infiniopKVCacheAppendDescriptor_t],
+    "infiniopCreatePagedAttentionDescriptor": [infiniopHandle_t, POINTER(infiniopPagedAttentionDescriptor_t)] + [infiniopTensorDescriptor_t] * 9
+                                              + [c_uint64, c_float],
+    "infiniopGetPagedAttentionWorkspaceSize": [infiniopPagedAttentionDescriptor_t, POINTER(c_uint64)],
+    "infiniopPagedAttention": [infiniopPagedAttentionDescriptor_t, c_void_p, c_uint64] + [c_void_p] * 10,
+    "infiniopDestroyPagedAttentionDescriptor": [infiniopPagedAttentionDescriptor_t],
+    "infiniopCreateKVCacheCopyDescriptor": [infiniopHandle_t, POINTER(infiniopKVCacheCopyDescriptor_t)] + [infiniopTensorDescriptor_t] * 5,
+    "infiniopKVCacheCopy": [infiniopKVCacheCopyDescriptor_t] + [c_void_p] * 6,
+    "infiniopDestroyKVCacheCopyDescriptor": [infiniopKVCacheCopyDescriptor_t],
+    "infiniopCreatePageTableUpdateDescriptor": [infiniopHandle_t, POINTER(infiniopPageTableUpdateDescriptor_t)] + [infiniopTensorDescriptor_t] * 10
+                                               + [c_uint64],
+    "infiniopGetPageTableUpdateWorkspaceSize": [infiniopPageTableUpdateDescriptor_t, POINTER(c_uint64)],
+    "infiniopPageTableUpdate": [infiniopPageTableUpdateDescriptor_t, c_void_p, c_uint64] + [c_void_p] * 11,
+    "infiniopDestroyPageTableUpdateDescriptor": [infiniopPageTableUpdateDescriptor_t],
+    "infiniopCreatePageTableCompactDescriptor": [infiniopHandle_t, POINTER(infiniopPageTableCompactDescriptor_t)] + [infiniopTensorDescriptor_t] * 7
+                                                + [c_uint64],
+    "infiniopGetPageTableCompactWorkspaceSize": [infiniopPageTableCompactDescriptor_t, POINTER(c_uint64)],
+    "infiniopPageTableCompact": [infiniopPageTableCompactDescriptor_t, c_void_p, c_uint64] + [c_void_p] * 8,
+    "infiniopDestroyPageTableCompactDescriptor": [infiniopPageTableCompactDescriptor_t],
+}
+
+PAGED_SYMBOLS = tuple(_PAGED_PROTOTYPES)
+
 
 # Entry points of this library that the reference does not have.
 EXTENSION_SYMBOLS = tuple(n for n in _PROTOTYPES if "AddRMSNorm" in n or "NoAlloc" in n)
@@ -175,9 +231,11 @@ def bind_prototypes(lib, extensions=True):
     """Attach argument and result types for every entry point.  Works on any
     library exporting the same C ABI: this one, or (with extensions=False) a
     build of the reference, which lacks the fused operator."""
-    for name, argtypes in _PROTOTYPES.items():
-        if not extensions and name in EXTENSION_SYMBOLS:
-            continue
+    return _bind(lib, {name: argtypes for name, argtypes in _PROTOTYPES.items() if extensions or name not in EXTENSION_SYMBOLS})
+
+
+def _bind(lib, prototypes):
+    for name, argtypes in prototypes.items():
         fn = getattr(lib, name)  # AttributeError names the missing symbol
         fn.argtypes = argtypes
         fn.restype = c_int32
@@ -188,7 +246,15 @@ _cached = {}
 
 
 def open_lib(path=None):
-    path = path or library_path()
+    return _open(path or library_path(), bind_prototypes)
+
+
+def open_paged_lib(path=None):
+    """libinfiniop_paged.so; handles and tensor descriptors are made with open_lib()'s library."""
+    return _open(path or library_path(PAGED_LIB_NAME), lambda lib: _bind(lib, _PAGED_PROTOTYPES))
+
+
+def _open(path, bind):
     if path in _cached:
         return _cached[path]
     # PyTorch-ROCm ships its own copy of the HIP runtime (same SONAME as the
@@ -203,6 +269,6 @@ def open_lib(path=None):
         raise FileNotFoundError(
             f"{path} not found: build it with `python -m operators_amd.build` "
             "or point INFINI_ROOT at an installed copy")
-    lib = bind_prototypes(ctypes.CDLL(path))
+    lib = bind(ctypes.CDLL(path))
     _cached[path] = lib
     return lib

@@ -18,13 +18,19 @@ from .liboperators import (
     infiniopRearrangeDescriptor_t,
     infiniopAddRMSNormDescriptor_t,
     infiniopAttentionDescriptor_t,
+    infiniopKVCacheAppendDescriptor_t,
+    infiniopKVCacheCopyDescriptor_t,
     infiniopMatmulDescriptor_t,
     infiniopMLPDescriptor_t,
+    infiniopPagedAttentionDescriptor_t,
+    infiniopPageTableCompactDescriptor_t,
+    infiniopPageTableUpdateDescriptor_t,
     infiniopRMSNormDescriptor_t,
     infiniopRandomSampleDescriptor_t,
     infiniopRoPEDescriptor_t,
     infiniopSwiGLUDescriptor_t,
     open_lib,
+    open_paged_lib,
 )
 from .utils import check_error, create_handle, destroy_handle, destroy_tensor, to_tensor
 
@@ -328,6 +334,119 @@ class RearrangePlan(_Plan):
         return dst
 
 
+class _PagedPlan(_Plan):
+    """A plan of libinfiniop_paged.so; owns the workspace its operator asks for (none: `_size` is None)."""
+
+    _create = _size = _descriptor = None
+
+    def __init__(self, ctx, tensors, *params):
+        import torch
+
+        super().__init__(ctx)
+        self.paged = open_paged_lib()
+        cts = self._describe(*tensors)
+        desc = self._descriptor()
+        try:
+            check_error(getattr(self.paged, self._create)(ctx.handle, ctypes.byref(desc), *[ct.descriptor for ct in cts], *params))
+        finally:
+            self._release(cts)
+        self.desc = desc
+        self.workspace_size, self.workspace = 0, None
+        if self._size is not None:
+            size = ctypes.c_uint64(0)
+            check_error(getattr(self.paged, self._size)(desc, ctypes.byref(size)))
+            self.workspace_size = size.value
+            if size.value:
+                self.workspace = torch.empty(size.value, dtype=torch.uint8, device=tensors[0].device)
+
+    def _space(self):
+        return (self.workspace.data_ptr() if self.workspace is not None else None), self.workspace_size
+
+    def close(self):
+        if self.desc is not None:
+            check_error(getattr(self.paged, self._destroy)(self.desc))
+            self.desc = None
+
+
+class KVCacheAppendPlan(_PagedPlan):
+    """k, v [tokens, kv_heads, dim] of every row's new tokens, rounded to 8 bits, into the pages of its `table` row.
+    Caches [pages, kv_heads, page, dim] (int8 or float8_e4m3fn), scales [pages, kv_heads, page / block] fp32,
+    table [rows, cols], offsets [rows + 1] and lengths [rows] int32 (include/infiniop_paged.h)."""
+
+    _create, _destroy = "infiniopCreateKVCacheAppendDescriptor", "infiniopDestroyKVCacheAppendDescriptor"
+    _size, _descriptor = "infiniopGetKVCacheAppendWorkspaceSize", infiniopKVCacheAppendDescriptor_t
+
+    def __init__(self, ctx, k_cache, v_cache, k_scale, v_scale, k, v, table, offsets, lengths):
+        super().__init__(ctx, (k_cache, v_cache, k_scale, v_scale, k, v, table, offsets, lengths))
+
+    def __call__(self, k_cache, v_cache, k_scale, v_scale, k, v, table, offsets, lengths, stream=None):
+        check_error(self.paged.infiniopKVCacheAppend(self.desc, *self._space(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                                                     v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), offsets.data_ptr(),
+                                                     lengths.data_ptr(), stream))
+
+
+class PagedAttentionPlan(_PagedPlan):
+    """out, q [tokens, heads, dim]: attention of every row's new tokens over the row's pages, causal among themselves.
+    max_tokens: the most new tokens of a row; scale: 1 / sqrt(dim) unless given."""
+
+    _create, _destroy = "infiniopCreatePagedAttentionDescriptor", "infiniopDestroyPagedAttentionDescriptor"
+    _size, _descriptor = "infiniopGetPagedAttentionWorkspaceSize", infiniopPagedAttentionDescriptor_t
+
+    def __init__(self, ctx, out, q, k_cache, v_cache, k_scale, v_scale, table, offsets, lengths, max_tokens, scale=None):
+        super().__init__(ctx, (out, q, k_cache, v_cache, k_scale, v_scale, table, offsets, lengths), max_tokens,
+                         q.shape[-1] ** -0.5 if scale is None else scale)
+
+    def __call__(self, out, q, k_cache, v_cache, k_scale, v_scale, table, offsets, lengths, stream=None):
+        check_error(self.paged.infiniopPagedAttention(self.desc, *self._space(), out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                                      k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(), offsets.data_ptr(), lengths.data_ptr(),
+                                                      stream))
+        return out
+
+
+class KVCacheCopyPlan(_PagedPlan):
+    """Pages pairs[i, 0] of a cache to pages pairs[i, 1], codes and scales; pairs [count, 2] int32, -1 for none."""
+
+    _create, _destroy = "infiniopCreateKVCacheCopyDescriptor", "infiniopDestroyKVCacheCopyDescriptor"
+    _descriptor = infiniopKVCacheCopyDescriptor_t
+
+    def __init__(self, ctx, k_cache, v_cache, k_scale, v_scale, pairs):
+        super().__init__(ctx, (k_cache, v_cache, k_scale, v_scale, pairs))
+
+    def __call__(self, k_cache, v_cache, k_scale, v_scale, pairs, stream=None):
+        check_error(self.paged.infiniopKVCacheCopy(self.desc, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                                   pairs.data_ptr(), stream))
+
+
+class PageTableUpdatePlan(_PagedPlan):
+    """Rows take over the pages of row source[r] (-1: none), then grow by grow[r] tokens; pairs [rows, 2]: pages to copy,
+    result [2]: pages lacking, rows too wide.  All int32; the new tensors may be the old ones."""
+
+    _create, _destroy = "infiniopCreatePageTableUpdateDescriptor", "infiniopDestroyPageTableUpdateDescriptor"
+    _size, _descriptor = "infiniopGetPageTableUpdateWorkspaceSize", infiniopPageTableUpdateDescriptor_t
+
+    def __init__(self, ctx, new_table, new_lengths, new_refcount, pairs, result, table, lengths, refcount, source, grow, page_size):
+        super().__init__(ctx, (new_table, new_lengths, new_refcount, pairs, result, table, lengths, refcount, source, grow), page_size)
+
+    def __call__(self, new_table, new_lengths, new_refcount, pairs, result, table, lengths, refcount, source, grow, stream=None):
+        check_error(self.paged.infiniopPageTableUpdate(self.desc, *self._space(), new_table.data_ptr(), new_lengths.data_ptr(), new_refcount.data_ptr(),
+                                                       pairs.data_ptr(), result.data_ptr(), table.data_ptr(), lengths.data_ptr(), refcount.data_ptr(),
+                                                       source.data_ptr(), grow.data_ptr(), stream))
+
+
+class PageTableCompactPlan(_PagedPlan):
+    """Renumbers the used pages to the lowest numbers; pairs [at least pages // 2, 2]: pages to copy, result [2]: used, moved."""
+
+    _create, _destroy = "infiniopCreatePageTableCompactDescriptor", "infiniopDestroyPageTableCompactDescriptor"
+    _size, _descriptor = "infiniopGetPageTableCompactWorkspaceSize", infiniopPageTableCompactDescriptor_t
+
+    def __init__(self, ctx, new_table, new_refcount, pairs, result, table, lengths, refcount, page_size):
+        super().__init__(ctx, (new_table, new_refcount, pairs, result, table, lengths, refcount), page_size)
+
+    def __call__(self, new_table, new_refcount, pairs, result, table, lengths, refcount, stream=None):
+        check_error(self.paged.infiniopPageTableCompact(self.desc, *self._space(), new_table.data_ptr(), new_refcount.data_ptr(), pairs.data_ptr(),
+                                                        result.data_ptr(), table.data_ptr(), lengths.data_ptr(), refcount.data_ptr(), stream))
+
+
 class Context:
     """A library handle on one GPU plus one-shot forms of the four operators."""
 
@@ -397,6 +516,36 @@ class Context:
     def causal_softmax(self, y, stream=None, use_workspace=True):
         with CausalSoftmaxPlan(self, y) as plan:
             return plan(y, stream, use_workspace)
+
+    def kv_cache_append(self, k_cache, v_cache, k_scale, v_scale, k, v, table, offsets, lengths, stream=None):
+        with KVCacheAppendPlan(self, k_cache, v_cache, k_scale, v_scale, k, v, table, offsets, lengths) as plan:
+            plan(k_cache, v_cache, k_scale, v_scale, k, v, table, offsets, lengths, stream)
+
+    def paged_attention(self, out, q, k_cache, v_cache, k_scale, v_scale, table, offsets, lengths, max_tokens, scale=None, stream=None):
+        import torch
+
+        with PagedAttentionPlan(self, out, q, k_cache, v_cache, k_scale, v_scale, table, offsets, lengths, max_tokens, scale) as plan:
+            plan(out, q, k_cache, v_cache, k_scale, v_scale, table, offsets, lengths, stream)
+            torch.cuda.synchronize()  # the plan's workspace must outlive the work queued on it
+            return out
+
+    def kv_cache_copy(self, k_cache, v_cache, k_scale, v_scale, pairs, stream=None):
+        with KVCacheCopyPlan(self, k_cache, v_cache, k_scale, v_scale, pairs) as plan:
+            plan(k_cache, v_cache, k_scale, v_scale, pairs, stream)
+
+    def page_table_update(self, new_table, new_lengths, new_refcount, pairs, result, table, lengths, refcount, source, grow, page_size, stream=None):
+        import torch
+
+        with PageTableUpdatePlan(self, new_table, new_lengths, new_refcount, pairs, result, table, lengths, refcount, source, grow, page_size) as plan:
+            plan(new_table, new_lengths, new_refcount, pairs, result, table, lengths, refcount, source, grow, stream)
+            torch.cuda.synchronize()  # the plan's workspace must outlive the work queued on it
+
+    def page_table_compact(self, new_table, new_refcount, pairs, result, table, lengths, refcount, page_size, stream=None):
+        import torch
+
+        with PageTableCompactPlan(self, new_table, new_refcount, pairs, result, table, lengths, refcount, page_size) as plan:
+            plan(new_table, new_refcount, pairs, result, table, lengths, refcount, stream)
+            torch.cuda.synchronize()  # the plan's workspace must outlive the work queued on it
 
     def rope(self, t, pos_ids, sin_table, cos_table, stream=None):
         with RoPEPlan(self, t, pos_ids, sin_table, cos_table) as plan:

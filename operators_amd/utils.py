@@ -39,7 +39,7 @@ def torch_dtype_to_layout(dtype):
     table = {
         torch.int8: dl.I8, torch.int16: dl.I16, torch.int32: dl.I32, torch.int64: dl.I64,
         torch.uint8: dl.U8, torch.float16: dl.F16, torch.bfloat16: dl.BF16,
-        torch.float32: dl.F32, torch.float64: dl.F64,
+        torch.float32: dl.F32, torch.float64: dl.F64, torch.float8_e4m3fn: dl.F8E4M3,
     }
     for name, layout in (("uint16", dl.U16), ("uint32", dl.U32), ("uint64", dl.U64)):
         if hasattr(torch, name):

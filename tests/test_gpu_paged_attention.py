@@ -1,0 +1,291 @@
+"""PagedAttention on the GPU against attention in 64 bits over the values that
+the codes stand for, element by element within what its roundings allow
+(paged_ref.attention_bound)."""
+import pytest
+import torch
+
+import paged_ref as ref
+from test_gpu_paged_cache import batch_of, make_cache, place
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+class Problem:
+    def __init__(self, rows, *, heads=8, kv_heads=2, dim=128, page=32, block=16, cache="i8", dtype="f16", layout="dense", seed=0, q_scale=2.0, behind=3,
+                 garbage=True, spread=0):
+        self.rows, self.heads, self.kv, self.dim, self.page, self.cache, self.dtype = rows, heads, kv_heads, dim, page, cache, dtype
+        pages = sum(-(-(a + b) // page) for a, b in rows) + 2
+        cols = max(-(-(a + b) // page) for a, b in rows) + 2
+        self.table, self.offsets, self.lengths = batch_of(rows, page, cols, pages, seed)
+        self.sides, self.gpu = [], []
+        for i in range(2):
+            codes, scales = make_cache(pages, kv_heads, page, dim, block, cache, seed + i)
+            if spread:
+                g = torch.Generator().manual_seed(seed + 7 + i)
+                scales = scales * torch.exp2(torch.randint(-spread, spread + 1, scales.shape, generator=g).float())
+            if garbage:  # what lies behind a row's end may be anything: NaN codes, and NaN scales where a whole block does
+                for r, (a, b) in enumerate(rows):
+                    n = a + b
+                    for pos in range(n, -(-n // page) * page):
+                        p = int(self.table[r, pos // page])
+                        codes.view(torch.uint8)[p, :, pos % page] = 0x7F if pos % 2 else 0xFF
+                        if pos % block == 0:
+                            scales[p, :, pos % page // block] = float("nan")
+                unused = set(range(pages)) - set(self.table.flatten().tolist())
+                for p in unused:
+                    codes.view(torch.uint8)[p] = 0x7F
+                    scales[p] = float("nan")
+            self.sides.append(ref.Cache(codes, scales, cache))
+            self.gpu.append((place(codes, layout), scales.to(DEV)))
+        g = torch.Generator().manual_seed(seed + 5)
+        self.q = (torch.randn(int(self.offsets[-1]) + behind, heads, dim, generator=g) * q_scale).to(ref.FLOAT[dtype])
+        self.scale = dim ** -0.5
+
+    def args(self):
+        (kc, ks), (vc, vs) = self.gpu
+        return kc, vc, ks, vs, self.table.to(DEV), self.offsets.to(DEV), self.lengths.to(DEV)
+
+    def run(self, ctx, max_tokens=None, q=None, out=None, stream=None):
+        q = self.q.to(DEV) if q is None else q
+        out = torch.full_like(self.q, 77.0, device=DEV) if out is None else out
+        most = max(b for _, b in self.rows) if max_tokens is None else max_tokens
+        ctx.paged_attention(out, q, *self.args(), max(most, 1), self.scale, stream)
+        torch.cuda.synchronize()
+        return out
+
+    def check(self, out, rows=None, most=None):
+        out = out.cpu()
+        for r, (had, new) in enumerate(self.rows):
+            if rows is not None and r not in rows:
+                continue
+            lo, n = int(self.offsets[r]), had + new
+            k, v = (s.read(self.table[r].tolist(), n) for s in self.sides)
+            there = ~k[:, 0, 0].isnan()
+            want, mean, size = ref.attention(self.q[lo:lo + new], k, v, self.scale, there)
+            got = out[lo:lo + new].double()
+            upto = new if most is None else min(new, most)
+            bound = ref.attention_bound(want, mean, size, self.dtype, self.dim, n, self.sides[1].top(self.table[r].tolist(), n))
+            off = ((got - want).abs() - bound)[:upto]
+            assert torch.isfinite(got[:upto]).all(), ("not finite", r)
+            assert (off <= 0).all(), (r, had, new, float(off.max()), float(((got - want).abs() / bound)[:upto].max()))
+            assert (out[lo + upto:lo + new] == 77.0).all(), ("beyond max_tokens", r)
+        assert (out[int(self.offsets[-1]):] == 77.0).all(), "rows behind the last sequence"
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 33, 127, 300, 1025, 5000])
+def test_decode_lengths(ctx, cache, dtype, length):
+    p = Problem([(length - 1, 1)], cache=cache, dtype=dtype, seed=length)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [16, 32, 64, 80, 96, 112, 128, 144, 160, 176, 192, 208, 240, 256])
+def test_head_widths(ctx, cache, dim):
+    p = Problem([(70, 1), (0, 3), (200, 2)], cache=cache, dtype="bf16", dim=dim, seed=dim)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("heads, kv_heads", [(1, 1), (5, 5), (8, 1), (7, 1), (16, 2), (40, 8), (17, 1), (48, 1), (6, 2)])
+@pytest.mark.parametrize("new", [1, 3, 9])
+def test_head_groups(ctx, heads, kv_heads, new):
+    p = Problem([(50, new), (333, 1), (0, new)], heads=heads, kv_heads=kv_heads, dim=64, cache="e4m3", dtype="f16", seed=heads)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("page, block", [(16, 16), (48, 16), (48, 48), (64, 32), (128, 128), (256, 64), (512, 512)])
+def test_pages_and_blocks(ctx, page, block):
+    p = Problem([(page - 1, 1), (page, 1), (5 * page + 7, 2), (0, 1)], page=page, block=block, dim=64, cache="i8", dtype="bf16", seed=page)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("new", [2, 5, 16, 33, 64, 100, 129, 257, 700])
+def test_prompts(ctx, cache, new):
+    p = Problem([(0, new), (300, new)], cache=cache, dtype="bf16", heads=8, kv_heads=2, dim=128, seed=new)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("dim", [16, 64, 80, 128, 144, 160, 192, 256])
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+def test_prompt_head_widths(ctx, cache, dim):
+    p = Problem([(37, 150), (0, 1), (500, 1), (0, 90)], cache=cache, dtype="f16", dim=dim, heads=6, kv_heads=2, seed=dim)
+    p.check(p.run(ctx))
+
+
+def test_mixed_batch_with_empty_rows(ctx):
+    rows = [(0, 0), (1000, 1), (200, 180), (5, 0), (0, 1), (0, 64), (64, 0), (2047, 1), (15, 17)]
+    for cache in ("i8", "e4m3"):
+        p = Problem(rows, cache=cache, dtype="bf16", heads=16, kv_heads=2, dim=64, seed=9)
+        p.check(p.run(ctx))
+
+
+def test_many_rows(ctx):
+    rows = [((37 * r) % 90, 0 if r % 13 == 5 else 1) for r in range(600)]
+    p = Problem(rows, heads=2, kv_heads=1, dim=16, page=16, cache="e4m3", seed=4)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("layout", ["tokens first", "wide"])
+@pytest.mark.parametrize("new", [1, 130])
+def test_layouts(ctx, layout, new):
+    p = Problem([(100, new), (30, 1)], layout=layout, dim=80, heads=6, kv_heads=3, cache="e4m3", dtype="bf16")
+    # q is a slice of a fused buffer at an odd place, out lies heads first
+    whole = torch.zeros(p.q.shape[0], 11, 81, dtype=p.q.dtype, device=DEV)
+    q = whole[:, 2:8, 1:]
+    q.copy_(p.q)
+    out = torch.full((6, p.q.shape[0], 80), 77.0, dtype=p.q.dtype, device=DEV).transpose(0, 1)
+    p.check(p.run(ctx, q=q, out=out))
+
+
+def test_max_tokens_leaves_the_rest(ctx):
+    p = Problem([(10, 5), (40, 2), (0, 90)], dim=64)
+    p.check(p.run(ctx, max_tokens=3), most=3)
+    p.check(p.run(ctx, max_tokens=1), most=1)
+    p.check(p.run(ctx, max_tokens=60), most=60)
+    p.check(p.run(ctx, max_tokens=10 ** 6))
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_bad_pages_see_nothing(ctx, new):
+    """Entries that are no page: their tokens do not exist; a row without a page: zeros."""
+    p = Problem([(200, new), (100, new), (0, new)], dim=64, cache="e4m3", page=32)
+    p.table[0, 2], p.table[0, 4] = -1, 10 ** 6
+    p.table[1, :] = -5
+    p.table[2, 0] = 2 ** 31 - 1
+    out = p.run(ctx)
+    p.check(out)
+    lo = int(p.offsets[1])
+    assert (out[lo:lo + new] == 0).all()
+
+
+def test_more_new_tokens_than_the_row_has(ctx):
+    """Tokens at places below 0 see nothing."""
+    p = Problem([(0, 40), (0, 3)], dim=64)
+    p.lengths[0] = 25
+    out = p.run(ctx).cpu()
+    assert (out[:15] == 0).all()
+    k, v = (s.read(p.table[0].tolist(), 25) for s in p.sides)
+    want, mean, size = ref.attention(p.q[15:40], k, v, p.scale)
+    assert ((out[15:40].double() - want).abs() <= ref.attention_bound(want, mean, size, p.dtype, 64, 25, p.sides[1].top(p.table[0].tolist(), 25))).all()
+    p.lengths[0] = -3
+    assert (p.run(ctx)[:40] == 0).all()
+
+
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("q_scale", [0.0, 1e-6, 60.0, 3000.0])
+def test_score_magnitudes(ctx, q_scale, new):
+    """From equal weights to a softmax that takes one key only; bf16 carries q of any size."""
+    p = Problem([(700, new)], q_scale=q_scale, dim=128, cache="i8", dtype="bf16", seed=2)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("new", [1, 50])
+def test_scales_far_apart(ctx, new):
+    """Blocks whose scales differ by up to 2^24, falling and rising along the row, and blocks of zeros."""
+    p = Problem([(900, new)], dim=64, cache="e4m3", dtype="bf16", spread=12, q_scale=0.02, seed=3)
+    for s, (_, g) in zip(p.sides, p.gpu):
+        s.scales[int(p.table[0, 0])] = 0
+        s.scales[int(p.table[0, 3])] = 0
+        g.copy_(s.scales)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("rows", [[(20000, 1)], [(9999, 20)], [(30000, 1), (10, 1), (0, 5), (4000, 2)], [(6000, 200), (0, 3)]], ids=str)
+def test_rows_shared_by_workgroups(ctx, rows):
+    p = Problem(rows, heads=8, kv_heads=1, dim=64, page=64, block=64, cache="i8", dtype="bf16", seed=8)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_two_calls_give_the_same_bits(ctx, new):
+    p = Problem([(8000, new), (77, 1)], heads=8, kv_heads=1, dim=128, cache="e4m3", seed=6)
+    a, b = p.run(ctx), p.run(ctx)
+    assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("rows", [[(5000, 1), (40, 1)], [(3000, 65), (2, 1)]], ids=str)
+def test_captured_and_replayed_with_other_lengths(ctx, rows):
+    """One graph serves whatever the index tensors hold at replay; eager calls and synchronisations in between."""
+    from operators_amd.ops import PagedAttentionPlan
+
+    p = Problem(rows, heads=8, kv_heads=2, dim=64, cache="e4m3", dtype="bf16", seed=1, garbage=False)
+    kc, vc, ks, vs, table, offsets, lengths = p.args()
+    q, out = p.q.to(DEV), torch.full_like(p.q, 77.0, device=DEV)
+    most = max(b for _, b in rows)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with PagedAttentionPlan(ctx, out, q, kc, vc, ks, vs, table, offsets, lengths, most, p.scale) as plan:
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            plan(out, q, kc, vc, ks, vs, table, offsets, lengths, stream=torch.cuda.current_stream().cuda_stream)
+        full = list(rows)
+        for cut in (0, 33, 1000, 0):
+            p.rows = [(max(0, full[0][0] - cut), full[0][1]), full[1]]
+            p.lengths = torch.tensor([a + b for a, b in p.rows], dtype=torch.int32)
+            lengths.copy_(p.lengths)
+            out.fill_(77.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            p.check(out)
+            assert torch.equal(p.run(ctx).view(torch.int16), out.view(torch.int16))
+
+
+def test_two_calls_at_once_with_workspaces_of_their_own(ctx):
+    from operators_amd.ops import PagedAttentionPlan
+
+    ps = [Problem([(9000 + 100 * i, 1)], heads=8, kv_heads=1, dim=128, cache="i8", seed=i) for i in range(3)]
+    streams = [torch.cuda.Stream() for _ in ps]
+    calls = []
+    for p in ps:
+        q, out = p.q.to(DEV), torch.full_like(p.q, 77.0, device=DEV)
+        a = p.args()
+        calls.append((PagedAttentionPlan(ctx, out, q, *a, 1, p.scale), out, q, a))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, (plan, out, q, a) in zip(streams, calls):
+            plan(out, q, *a, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for p, (plan, out, _, _) in zip(ps, calls):
+        p.check(out)
+        plan.close()
+
+
+def test_workspace_and_pointer_refusals(ctx):
+    from operators_amd import InfiniopError
+    from operators_amd.ops import PagedAttentionPlan
+
+    p = Problem([(30, 1)], dim=64)
+    a, q = p.args(), p.q.to(DEV)
+    out = torch.empty_like(q)
+    with PagedAttentionPlan(ctx, out, q, *a, 1) as plan:
+        args = [t.data_ptr() for t in (out, q, *a)]
+        call = plan.paged.infiniopPagedAttention
+        assert call(plan.desc, plan.workspace.data_ptr(), plan.workspace_size - 1, *args, None) == 6
+        assert call(plan.desc, None, plan.workspace_size, *args, None) == 6
+        for i in range(len(args)):
+            assert call(plan.desc, plan.workspace.data_ptr(), plan.workspace_size, *args[:i], None, *args[i + 1:], None) == 2, i
+        for i in (2, 3):
+            assert call(plan.desc, plan.workspace.data_ptr(), plan.workspace_size, *args[:i], args[i] + 8, *args[i + 1:], None) == 2, i
+        assert call(plan.desc, plan.workspace.data_ptr() + 4, plan.workspace_size, *args, None) == 2
+    with pytest.raises(InfiniopError):
+        PagedAttentionPlan(ctx, out, q[:, :5], *a, 1)
+    torch.cuda.synchronize()
+
+
+def test_random_problems(ctx):
+    import random
+
+    rng = random.Random(77)
+    for trial in range(40):
+        kv = rng.choice([1, 2, 3, 8])
+        rows = [(rng.choice([0, rng.randint(0, 100), rng.randint(0, 3000)]), rng.choice([0, 1, 1, 2, rng.randint(1, 200)])) for _ in range(rng.randint(1, 6))]
+        if not any(a + b for a, b in rows):
+            rows.append((3, 1))
+        page = rng.choice([16, 32, 48, 64, 128])
+        p = Problem(rows, heads=kv * rng.choice([1, 2, 5, 8]), kv_heads=kv, dim=16 * rng.randint(1, 16), page=page, block=rng.choice([b for b in (16, 32, 48, 64, 128) if page % b == 0]),
+                    cache=rng.choice(["i8", "e4m3"]), dtype=rng.choice(["f16", "bf16"]), layout=rng.choice(["dense", "tokens first", "wide"]), seed=trial)
+        print(trial, p.rows, p.heads, p.kv, p.dim, p.page, p.cache, p.dtype, flush=True)
+        p.check(p.run(ctx))
