@@ -12,7 +12,7 @@
  * The cache of one layer is four tensors:
  *   k_cache, v_cache  [pages, kv_heads, page, dim]           I8 or F8E4M3 codes
  *   k_scale, v_scale  [pages, kv_heads, page / block]        F32
- * and stands for code * scale, one scale for each `block` tokens of a head.
+ * and stands for code * scale, one scale (not below 0) for each `block` tokens of a head.
  * page and block are multiples of 16 (block divides page), dim is a multiple of
  * 16 up to 256.  The innermost strides are 1, the others free: codes in
  * multiples of 16, so the pages of all heads may lie in any order, e.g. as

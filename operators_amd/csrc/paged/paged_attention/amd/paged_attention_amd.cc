@@ -5,7 +5,14 @@
 
 namespace {
 
-uint32_t padded(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 && dim % 48 == 0 ? 192 : 256; }
+// Sequences of up to this many query rows go to the kernel for decoding.
+constexpr uint32_t kFewRows = 32;
+
+// Only tiles of several units use the workspace: of those, a tile of k keys is cut at every c of them where the sum of
+// all k is at most target * c, so they are at most 2 target units of a head (ceil(x) <= 2 x from 1 on).
+uint64_t workspace_of(const PagedAttentionShape &s, const amd::PagedCache &c) {
+    return s.most_tiles == 0 ? 0 : 2ull * s.target * c.kv_heads * s.tile_rows * (paged_dim(c.dim) + 2) * sizeof(float);
+}
 
 }// namespace
 
@@ -44,24 +51,28 @@ infiniopStatus_t amdCreatePagedAttentionDescriptor(AmdHandle_t handle, PagedAtte
     }
     if (max_tokens > tokens) max_tokens = tokens;
 
-    PagedAttentionShape shape;
-    // (two sets of 16 rows share what they read; heads wider than 128 leave no registers for that)
-    shape.tile_rows = max_tokens * group <= 16 || cache.dim > 128 ? 16 : 32;
-    // every row with tokens has one tile that it does not fill
-    const uint64_t busy = rows.rows < tokens ? rows.rows : tokens;
-    shape.most_tiles = static_cast<uint32_t>(tokens * group / shape.tile_rows + busy);
+    // a sequence with tokens has at most one tile that it does not fill
+    const uint64_t busy = rows.rows < tokens ? rows.rows : tokens, query_rows = tokens * group, most_rows = max_tokens * group;
+    PagedAttentionShape few{}, many{};
+    // two sets of 16 rows share what they read; heads wider than 128 leave no registers for that
+    few.tile_rows = most_rows <= 16 || cache.dim > 128 ? 16 : 32;
+    few.least = 1;
+    few.most = kFewRows;
+    few.most_tiles = static_cast<uint32_t>(query_rows / few.tile_rows + busy);
     // about three workgroups of a unit for each of the compute units
-    shape.target = static_cast<uint32_t>(amd::ceil_div(3ull * handle->cu_count, cache.kv_heads));
-    if ((static_cast<uint64_t>(shape.target) + shape.most_tiles) * cache.kv_heads > amd::max_grid_1d(256)) {
-        return STATUS_BAD_TENSOR_SHAPE;
+    few.target = static_cast<uint32_t>(amd::ceil_div(3ull * handle->cu_count, cache.kv_heads));
+    many.tile_rows = 32 * paged_tile_waves(paged_dim(cache.dim));
+    many.least = kFewRows + 1;
+    many.most = UINT32_MAX;
+    many.most_tiles = most_rows <= kFewRows ? 0 : static_cast<uint32_t>(query_rows / many.tile_rows + busy);
+    many.target = static_cast<uint32_t>(amd::ceil_div(handle->cu_count, cache.kv_heads));
+    for (const PagedAttentionShape &s : {few, many}) {
+        if ((static_cast<uint64_t>(s.target) + s.most_tiles) * cache.kv_heads > amd::max_grid_1d(512)) return STATUS_BAD_TENSOR_SHAPE;
     }
-    // Only tiles of several units use the workspace: of those, a tile of k keys is cut at every c of them where the
-    // sum of all k is at most target * c, so they are at most 2 target units (ceil(x) <= 2 x from 1 on).
-    const uint64_t units = 2ull * shape.target * cache.kv_heads;
-    const uint64_t bytes = units * shape.tile_rows * (padded(cache.dim) + 2) * sizeof(float);
+    const uint64_t for_few = workspace_of(few, cache), for_many = workspace_of(many, cache), bytes = for_few > for_many ? for_few : for_many;
     auto *desc = new (std::nothrow) PagedAttentionAmdDescriptor{
         DevAmdGpu, handle->device_id, amd::same_dt(q->dt, BF16), cache, rows, static_cast<uint32_t>(tokens), static_cast<uint32_t>(group),
-        static_cast<uint32_t>(max_tokens), q->strides[0], q->strides[1], out->strides[0], out->strides[1], scale, shape,
+        static_cast<uint32_t>(max_tokens), q->strides[0], q->strides[1], out->strides[0], out->strides[1], scale, few, many,
         tokens == 0 || rows.rows == 0 ? 0 : bytes};
     if (desc == nullptr) {
         return STATUS_MEMORY_NOT_ALLOCATED;

@@ -4,14 +4,22 @@
 
 #include "../../paged_cache.h"
 
+// The width that the kernels hold a head in.  192 for those that whole lanes of 12 columns make up.
+constexpr uint32_t paged_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 && dim % 48 == 0 ? 192 : 256; }
+// Wavefronts of 32 query rows each that a workgroup of the kernel for prompts has.
+constexpr int paged_tile_waves(int padded) { return padded <= 128 ? 8 : 4; }
+
 // How a call's work is cut up.  A tile is up to `tile_rows` query rows (token by
 // head of one K/V head's group) of one sequence; a unit is a tile over a range of
 // keys, and what one workgroup computes.  `target` units of a K/V head are aimed
-// at; a tile is split over several units where that gives fewer.
+// at; a tile is split over several units where that gives fewer.  Sequences with
+// at least `least` and at most `most` query rows are taken, the others left to the
+// other kernel.
 struct PagedAttentionShape {
     uint32_t tile_rows;
-    uint32_t most_tiles;// of one K/V head, whatever the offsets
+    uint32_t most_tiles;// of one K/V head, whatever the offsets; 0: the kernel is not needed
     uint32_t target;
+    uint32_t least, most;
 };
 
 struct PagedAttentionAmdDescriptor {
@@ -23,7 +31,7 @@ struct PagedAttentionAmdDescriptor {
     uint32_t tokens, group, max_tokens;
     int64_t q_token, q_head, out_token, out_head;// elements
     float scale;
-    PagedAttentionShape shape;
+    PagedAttentionShape few, many;// query rows: decoding, prompts
     uint64_t workspace;
 };
 typedef PagedAttentionAmdDescriptor *PagedAttentionAmdDescriptor_t;

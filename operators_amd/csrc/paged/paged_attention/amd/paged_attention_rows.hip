@@ -415,60 +415,85 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_join(AttentionA
     Unit u;
     const uint32_t head = blockIdx.x % a.kv_heads;
     if (!find_unit<kWaves, true>(a, blockIdx.x / a.kv_heads, slots, &shared_unit, &u)) return;
-    const uint32_t lane = threadIdx.x & (kWave - 1), in_tile = blockIdx.y * kWaves + threadIdx.x / kWave;
-    const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens;
-    const uint32_t r = u.tile * a.tile_rows + in_tile;
-    if (r >= tokens * a.group) return;
-    const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * a.tile_rows + in_tile; };
-    float high = kNone;
-    for (uint32_t c = lane; c < u.chunks; c += kWave) high = fmaxf(high, a.part_stat[2 * at(c)]);
-    high = wave_max(high);
-    float total = 0.0f, o[PER] = {};
-    for (uint32_t base = 0; base < u.chunks; base += kWave) {
-        const uint32_t mine = base + lane;
-        float by = 0.0f, l = 0.0f;
-        if (mine < u.chunks) {
-            l = a.part_stat[2 * at(mine) + 1];
-            by = l > 0.0f ? __builtin_amdgcn_exp2f(a.part_stat[2 * at(mine)] - high) : 0.0f;
-        }
-        total += wave_sum(l * by);
-        const uint32_t n = u.chunks - base < kWave ? u.chunks - base : kWave;
-        for (uint32_t c = 0; c < n; ++c) {
-            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, by), c));
-            if (w == 0.0f) continue;// (a unit that saw nothing has written nothing)
-            const float *p = a.part_out + at(base + c) * DP + lane * PER;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave)));
+    const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens, row0 = u.tile * a.tile_rows, left = tokens * a.group - row0;
+    const uint32_t rows = left < a.tile_rows ? left : a.tile_rows;
+    for (uint32_t in_tile = blockIdx.y * kWaves + wave; in_tile < rows; in_tile += gridDim.y * kWaves) {
+        const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * a.tile_rows + in_tile; };
+        float high = kNone;
+        for (uint32_t c = lane; c < u.chunks; c += kWave) high = fmaxf(high, a.part_stat[2 * at(c)]);
+        high = wave_max(high);
+        float total = 0.0f, o[PER] = {};
+        for (uint32_t base = 0; base < u.chunks; base += kWave) {
+            const uint32_t mine = base + lane;
+            float by = 0.0f, l = 0.0f;
+            if (mine < u.chunks) {
+                l = a.part_stat[2 * at(mine) + 1];
+                by = l > 0.0f ? __builtin_amdgcn_exp2f(a.part_stat[2 * at(mine)] - high) : 0.0f;
+            }
+            total += wave_sum(l * by);
+            const uint32_t n = u.chunks - base < kWave ? u.chunks - base : kWave;
+            for (uint32_t c = 0; c < n; ++c) {
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, by), c));
+                if (w == 0.0f) continue;// (a unit that saw nothing has written nothing)
+                const float *p = a.part_out + at(base + c) * DP + lane * PER;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) o[i] += w * p[i];
+                for (int i = 0; i < PER; ++i) o[i] += w * p[i];
+            }
         }
-    }
-    const float by = total > 0.0f ? 1.0f / total : 0.0f;
-    const uint32_t token = fast_quotient(r, a.by_group);
-    uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + static_cast<int64_t>(head * a.group + (r - token * a.group)) * a.out_head;
+        const float by = total > 0.0f ? 1.0f / total : 0.0f;
+        const uint32_t r = row0 + in_tile, token = fast_quotient(r, a.by_group);
+        uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + static_cast<int64_t>(head * a.group + (r - token * a.group)) * a.out_head;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        if (lane * PER + i < a.dim) p[lane * PER + i] = static_cast<uint16_t>(narrow2_rne(a.bf16, o[i] * by, 0.0f));
+        for (int i = 0; i < PER; ++i) {
+            if (lane * PER + i < a.dim) p[lane * PER + i] = static_cast<uint16_t>(narrow2_rne(a.bf16, o[i] * by, 0.0f));
+        }
     }
 }
 
+// The kernel for few query rows, the one for many, and after either what joins its units.
 template<bool FP8, int DP>
-void launch(const PagedAttentionAmdDescriptor &d, const AttentionArgs &a, hipStream_t s) {
-    const unsigned units = (d.shape.target + d.shape.most_tiles) * d.cache.kv_heads;
-    if constexpr (DP <= 128) {
-        if (d.shape.tile_rows == 16) paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
-        else paged_attention_rows<FP8, DP, 2><<<units, kWaves * kWave, 0, s>>>(a);
-    } else {
-        paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
+void launch(const PagedAttentionAmdDescriptor &d, AttentionArgs a, hipStream_t s) {
+    const auto shape = [&](const PagedAttentionShape &z) {
+        a.tile_rows = z.tile_rows;
+        a.by_tile = fast_div(z.tile_rows);
+        a.units_each = 1.0f / static_cast<float>(z.target);
+        a.least_rows = z.least;
+        a.most_rows = z.most;
+        // the workspace: statistics of all slots, then their sums
+        a.part_out = a.part_stat + 4ull * z.target * d.cache.kv_heads * z.tile_rows;
+        return (z.target + z.most_tiles) * d.cache.kv_heads;
+    };
+    {
+        const unsigned units = shape(d.few);
+        a.least_steps = 8;
+        a.whole_steps = 1;
+        if constexpr (DP <= 128) {
+            if (d.few.tile_rows == 16) paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
+            else paged_attention_rows<FP8, DP, 2><<<units, kWaves * kWave, 0, s>>>(a);
+        } else {
+            paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
+        }
+        // a tile of several units has two at least
+        paged_attention_join<DP><<<dim3(d.few.target * d.cache.kv_heads, d.few.tile_rows / kWaves), kWaves * kWave, 0, s>>>(a);
     }
-    // a tile of several units has two at least
-    paged_attention_join<DP><<<dim3(d.shape.target * d.cache.kv_heads, d.shape.tile_rows / kWaves), kWaves * kWave, 0, s>>>(a);
+    if (d.many.most_tiles != 0) {
+        const unsigned units = shape(d.many);
+        a.least_steps = 16;
+        a.whole_steps = 2;
+        amdLaunchPagedAttentionTiles(a, FP8, units, s);
+        paged_attention_join<DP><<<dim3(d.many.target * d.cache.kv_heads, 8), kWaves * kWave, 0, s>>>(a);
+    }
 }
 
 template<bool FP8>
 void launch(const PagedAttentionAmdDescriptor &d, const AttentionArgs &a, hipStream_t s) {
-    if (d.cache.dim <= 64) launch<FP8, 64>(d, a, s);
-    else if (d.cache.dim <= 128) launch<FP8, 128>(d, a, s);
-    else if (d.cache.dim <= 192 && d.cache.dim % 48 == 0) launch<FP8, 192>(d, a, s);// (12 columns a lane: whole lanes)
-    else launch<FP8, 256>(d, a, s);
+    switch (paged_dim(d.cache.dim)) {
+        case 64: return launch<FP8, 64>(d, a, s);
+        case 128: return launch<FP8, 128>(d, a, s);
+        case 192: return launch<FP8, 192>(d, a, s);
+        default: return launch<FP8, 256>(d, a, s);
+    }
 }
 
 }// namespace
@@ -490,38 +515,31 @@ infiniopStatus_t amdPagedAttention(PagedAttentionAmdDescriptor_t desc, void *wor
         return STATUS_BAD_PARAM;
     }
     AMD_CHECK_HIP(hipSetDevice(d.device_id), STATUS_BAD_DEVICE);
-    const uint64_t slots = 2ull * d.shape.target * d.cache.kv_heads * d.shape.tile_rows;
-    auto *parts = static_cast<float *>(workspace);
-    const AttentionArgs a{
-        {static_cast<const int *>(table), static_cast<const int *>(offsets), static_cast<const int *>(lengths), d.rows.stride, d.rows.rows, d.rows.cols,
-         d.tokens, d.cache.page, amd::fast_div(d.cache.page)},
-        static_cast<const uint8_t *>(k_cache),
-        static_cast<const uint8_t *>(v_cache),
-        static_cast<const float *>(k_scale),
-        static_cast<const float *>(v_scale),
-        d.cache.k,
-        d.cache.v,
-        static_cast<const uint16_t *>(q),
-        static_cast<uint16_t *>(out),
-        d.q_token,
-        d.q_head,
-        d.out_token,
-        d.out_head,
-        d.cache.pages,
-        d.cache.kv_heads,
-        d.cache.dim,
-        d.group,
-        d.max_tokens,
-        d.shape.tile_rows,
-        amd::fast_div(d.group),
-        amd::fast_div(d.cache.block),
-        amd::fast_div(d.shape.tile_rows),
-        d.scale * 1.44269504088896340736f,
-        1.0f / static_cast<float>(d.shape.target),
-        8,
-        d.bf16,
-        parts + 2 * slots,
-        parts};
+    AttentionArgs a{};
+    a.rows = amd::RaggedRows{static_cast<const int *>(table), static_cast<const int *>(offsets), static_cast<const int *>(lengths), d.rows.stride,
+                             d.rows.rows, d.rows.cols, d.tokens, d.cache.page, amd::fast_div(d.cache.page)};
+    a.k = static_cast<const uint8_t *>(k_cache);
+    a.v = static_cast<const uint8_t *>(v_cache);
+    a.k_scale = static_cast<const float *>(k_scale);
+    a.v_scale = static_cast<const float *>(v_scale);
+    a.k_at = d.cache.k;
+    a.v_at = d.cache.v;
+    a.q = static_cast<const uint16_t *>(q);
+    a.out = static_cast<uint16_t *>(out);
+    a.q_token = d.q_token;
+    a.q_head = d.q_head;
+    a.out_token = d.out_token;
+    a.out_head = d.out_head;
+    a.pages = d.cache.pages;
+    a.kv_heads = d.cache.kv_heads;
+    a.dim = d.cache.dim;
+    a.group = d.group;
+    a.max_tokens = d.max_tokens;
+    a.by_group = amd::fast_div(d.group);
+    a.by_block = amd::fast_div(d.cache.block);
+    a.scale = d.scale * 1.44269504088896340736f;
+    a.bf16 = d.bf16;
+    a.part_stat = static_cast<float *>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
     d.cache.fp8 ? launch<true>(d, a, s) : launch<false>(d, a, s);
     AMD_CHECK_HIP(hipGetLastError(), STATUS_EXECUTION_FAILED);

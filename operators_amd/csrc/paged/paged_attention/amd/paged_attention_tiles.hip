@@ -1,0 +1,369 @@
+// gfx950 PagedAttention for many query rows: prompts and chunks of them.
+//     S = K q^T,  P = exp2(scale S - m),  O = V^T P^T      transposed as in paged_attention_rows.hip
+// A workgroup takes 256 query rows of one K/V head (tokens by heads of its group), a
+// wavefront 32 of them, and all walk the keys together, 64 at a time (heads wider than
+// 128: 128 rows, for one wavefront's registers are two's, and 32 keys).  A tile's codes
+// are turned into fp16 once for all wavefronts on their way into LDS, keys by columns for K, columns by keys for V, so that either
+// product reads its operand as 16-byte vectors; rows are 16 bytes longer than a power
+// of two, which spreads eight neighbouring lanes over all banks.  Two tiles lie in LDS:
+// while one is computed with, the next is written and the one behind it is on its way
+// from memory; one barrier a tile.
+// v_mfma_f32_32x32x16 leaves a lane 16 of the 32 keys of one query, and V's keys lie in
+// the order in which those make up the second product's operand, so P is not exchanged.
+// The V scale of a block is added to the exponent (P = exp2(x - m + log2 r)) and taken
+// out of its sum again (sum / r), which saves a product for each score.
+// Bound by the matrix units and, nearly as much, by the vector units (about 7 slots for
+// each score, 4 of them the exponential) and LDS (both operands for 32 rows a wavefront).
+#include "paged_attention_units.h"
+
+namespace {
+
+using namespace amd;
+
+constexpr float kLift = 10.0f, kSlack = 4.0f, kNone = -1.0e30f;// as in paged_attention_rows.hip
+constexpr float kLeastRatio = 0x1p-40f;// of a V scale to the largest: P times it is 0 in fp16
+
+__device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+
+template<bool FP8, int DP>
+__global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_tiles(AttentionArgs a) {
+    constexpr int kWaves = paged_tile_waves(DP), kLanes = kWaves * kWave;
+    constexpr int BK = DP <= 128 ? 64 : 32;        // keys of a tile
+    constexpr int KS = DP / 16, NC = DP / 16;      // steps of the first product; 16-byte pieces of a key
+    constexpr int TD = DP / 32, NB = BK / 32, NG = BK / 16;
+    constexpr int KP = DP * 2 + 16, VP = BK * 2 + 16;// bytes of a row in LDS
+    constexpr int K_TASKS = BK * NC, V_TASKS = BK / 4 * (DP / 4);
+    static_assert(K_TASKS == V_TASKS, "as many pieces of K as of V");
+    constexpr int PER = (K_TASKS + kLanes - 1) / kLanes;// of a lane
+    __shared__ __attribute__((aligned(16))) uint8_t k_lds[2][BK * KP];
+    __shared__ __attribute__((aligned(16))) uint8_t v_lds[2][DP * VP];
+    __shared__ uint64_t slots[kWaves];
+    __shared__ Unit shared_unit;
+    Unit u;
+    const uint32_t head = blockIdx.x % a.kv_heads;
+    if (!find_unit<kWaves, false>(a, blockIdx.x / a.kv_heads, slots, &shared_unit, &u)) return;
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tid / kWave)));
+    const uint32_t n32 = lane & 31u, h = lane >> 5;
+    const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens;
+    const uint32_t row0 = u.tile * a.tile_rows, rows = tokens * a.group;
+    const int seen = static_cast<int>(u.length) - static_cast<int>(u.count);
+    const auto sees = [&](uint32_t token) { return static_cast<uint32_t>(seen + static_cast<int>(token) < 0 ? 0 : seen + static_cast<int>(token) + 1); };
+    const uint32_t row_end = row0 + a.tile_rows < rows ? row0 + a.tile_rows : rows;
+    // this wavefront's rows, and what its first and its last see
+    const uint32_t mine0 = row0 + wave * 32, mine1 = mine0 + 32 < row_end ? mine0 + 32 : row_end;
+    const bool any = mine0 < row_end;
+    const uint32_t all_see = any ? sees(fast_quotient(mine0, a.by_group)) : 0, some_see = any ? sees(fast_quotient(mine1 - 1, a.by_group)) : 0;
+    const uint32_t tile_sees = sees(fast_quotient(row_end - 1, a.by_group));
+
+    const uint32_t r = mine0 + n32, token = fast_quotient(r, a.by_group);
+    const bool mine = r < row_end;
+    const uint32_t limit = mine ? sees(token) : 0;
+    const int64_t q_head = static_cast<int64_t>(head * a.group + (r - token * a.group));
+    // the query row as the second operand: piece 2 s + h of K's order in LDS at step s
+    f16x8 q[KS];
+    float factor;
+    {
+        u32x4 w[KS];
+        const uint16_t *p = a.q + static_cast<int64_t>(u.first + token) * a.q_token + q_head * a.q_head;
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const uint32_t piece = 2 * s + h, d = piece % NC * 16 + piece / NC * 8;
+            w[s] = u32x4{0, 0, 0, 0};
+            if (mine && d < a.dim) w[s] = ld16_any(p + d);
+            float x[8];
+            if (a.bf16) widen8<BF16Rne>(w[s], x);
+            else widen8<F16Ref>(w[s], x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+        }
+        top = pair_max(top);
+        const int e = top > 0.0f ? static_cast<int>(__float_as_uint(top) >> 23) - 127 : 0;
+        factor = ldexpf(fabsf(a.scale), e);// (its sign goes into q: the largest product is the largest score)
+        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            float x[8];
+            if (a.bf16) widen8<BF16Rne>(w[s], x);
+            else widen8<F16Ref>(w[s], x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[s][i] = static_cast<_Float16>(ldexpf(x[i] * sign, -e));
+        }
+    }
+    f32x16 o[TD];
+#pragma unroll
+    for (int t = 0; t < TD; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    }
+    float m = kNone, l = 0.0f, v_top = 0.0f, v_inv = 0.0f;
+
+    // a lane's pieces of a tile: 16 bytes of one key of K, 4 bytes of 4 keys of V
+    const auto k_key = [&](int i) { return (tid + i * kLanes) / NC; };
+    const auto k_piece = [&](int i) { return (tid + i * kLanes) % NC; };
+    const auto v_keys = [&](int i) { return (tid + i * kLanes) / (DP / 4) * 4; };
+    const auto v_col = [&](int i) { return (tid + i * kLanes) % (DP / 4) * 4; };
+    const auto works = [&](int i) { return K_TASKS % kLanes == 0 || tid + i * kLanes < K_TASKS; };
+    uint32_t k_off[PER], v_off[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        k_off[i] = (k_key(i) & 15u) * a.k_at.token + (k_piece(i) * 16 < a.dim ? k_piece(i) * 16 : 0);// (q is 0 behind dim)
+        v_off[i] = (v_keys(i) & 15u) * a.v_at.token + (v_col(i) < a.dim ? v_col(i) : 0);             // (not stored behind dim)
+    }
+    const uint8_t *k_base = a.k + static_cast<uint64_t>(head) * a.k_at.head, *v_base = a.v + static_cast<uint64_t>(head) * a.v_at.head;
+    const float *ks_base = a.k_scale + static_cast<int64_t>(head) * a.k_at.s_head, *vs_base = a.v_scale + static_cast<int64_t>(head) * a.v_at.s_head;
+    const int *table = a.rows.table + u.row * a.rows.stride;
+
+    const uint32_t end = (tile_sees + kStepKeys - 1) / kStepKeys;
+    const uint32_t s0 = u.chunk * u.steps, s1 = s0 + u.steps < end ? s0 + u.steps : end;
+    const uint32_t first_key = s0 * kStepKeys, tiles = s1 > s0 ? (s1 - s0 + NB - 1) / NB : 0;
+
+    // pages, places in them and scales of 64 groups of 16 keys, one for each lane: those of the tiles that are computed
+    // with, and those of the tiles that are loaded (which run ahead)
+    constexpr uint32_t kAhead = 64 / NG;// tiles of such a set
+    struct Groups {
+        int page;
+        uint32_t place;
+        float k_scale, v_scale;
+    };
+    const auto groups_of = [&](uint32_t tile) {
+        Groups g{-1, 0, 0.0f, 0.0f};
+        const uint32_t key = first_key + tile * BK + lane * 16;
+        if (key < u.length) {
+            const uint32_t col = fast_quotient(key, a.rows.by_page);
+            g.page = table[col];
+            g.place = key - col * a.rows.page;
+            if (static_cast<uint32_t>(g.page) < a.pages) {
+                const uint32_t block = fast_quotient(g.place, a.by_block);
+                g.k_scale = ks_base[g.page * a.k_at.s_page + block];
+                g.v_scale = vs_base[g.page * a.v_at.s_page + block];
+            } else {
+                g.page = -1;
+            }
+        }
+        return g;
+    };
+    const auto lane_of = [](float v, uint32_t l2) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l2)); };
+
+    u32x4 k_raw[PER];
+    uint32_t v_raw[PER][4];
+    int v_live[PER];// how many of the 4 keys there are
+    Groups ahead = groups_of(0), here = ahead;
+    const auto load = [&](uint32_t tile) {
+        if (tile % kAhead == 0 && tile != 0) ahead = groups_of(tile);
+        const uint32_t at = tile % kAhead * NG;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (!works(i)) continue;
+            // (the same group for the whole wavefront: 16 keys are the pieces of whole wavefronts, or a wavefront's are within 16 keys)
+            const uint32_t kg = at + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(k_key(i) / 16)));
+            const uint32_t vg = at + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v_keys(i) / 16)));
+            const int kp = __builtin_amdgcn_readlane(ahead.page, kg), vp = __builtin_amdgcn_readlane(ahead.page, vg);
+            const uint32_t k_place = __builtin_amdgcn_readlane(ahead.place, kg), v_place = __builtin_amdgcn_readlane(ahead.place, vg);
+            const uint8_t *k = k_base + static_cast<int64_t>(kp < 0 ? 0 : kp) * a.k_at.page + static_cast<uint64_t>(k_place) * a.k_at.token;
+            const uint8_t *v = v_base + static_cast<int64_t>(vp < 0 ? 0 : vp) * a.v_at.page + static_cast<uint64_t>(v_place) * a.v_at.token;
+            k_raw[i] = ld16(k + k_off[i]);
+            v_live[i] = vp < 0 ? 0 : static_cast<int>(u.length) - static_cast<int>(first_key + tile * BK + v_keys(i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v_raw[i][j] = *reinterpret_cast<const uint32_t *>(v + static_cast<uint64_t>(j) * a.v_at.token + v_off[i]);
+        }
+    };
+    const auto store = [&](uint32_t tile) {
+        const uint32_t buffer = tile & 1u;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (!works(i)) continue;
+            uint8_t *k = k_lds[buffer] + k_key(i) * KP + k_piece(i) * 16;
+            f16x8 lo, hi;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t c = prepare_codes<FP8>(k_raw[i][w]);
+                const f16x2 x = pair_of<FP8, false>(c), y = pair_of<FP8, true>(c);
+                f16x8 &to = w < 2 ? lo : hi;
+                to[w % 2 * 4] = x.x;
+                to[w % 2 * 4 + 1] = x.y;
+                to[w % 2 * 4 + 2] = y.x;
+                to[w % 2 * 4 + 3] = y.y;
+            }
+            *reinterpret_cast<f16x8 *>(k) = lo;
+            *reinterpret_cast<f16x8 *>(k + NC * 16) = hi;
+            uint32_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = v_raw[i][j];
+            // what lies behind the row's end, or in no page, may be anything: no number times 0 is 0
+            if (v_live[i] < 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = j >= v_live[i] ? 0 : x[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = prepare_codes<FP8>(x[j]);
+            uint32_t pair[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                pair[j][0] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05010400u);
+                pair[j][1] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07030602u);
+            }
+            // 16 keys in order of the accumulator's halves: 0-3, 8-11, 4-7, 12-15
+            const uint32_t quad = v_keys(i) / 4 & 3u, place = (v_keys(i) & ~15u) + (quad & 1u) * 8 + (quad >> 1) * 4;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const auto two = [&](int j) { return __builtin_bit_cast(uint32_t, c % 2 ? pair_of<FP8, true>(pair[j][c / 2]) : pair_of<FP8, false>(pair[j][c / 2])); };
+                // column d is row d / TD of the accumulator's tile d % TD
+                const uint32_t d = v_col(i) + c, row = d % TD * 32 + d / TD;
+                *reinterpret_cast<u32x2 *>(v_lds[buffer] + row * VP + place * 2) = u32x2{two(0), two(1)};
+            }
+        }
+    };
+
+    const auto compute = [&](uint32_t tile) {
+        const uint32_t key0 = first_key + tile * BK, buffer = tile & 1u;
+        if (tile % kAhead == 0 && tile != 0) here = groups_of(tile);
+        if (key0 >= some_see) return;
+        const uint32_t at = tile % kAhead * NG;
+        f32x16 s[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < KS; ++e) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const f16x8 x = *reinterpret_cast<const f16x8 *>(k_lds[buffer] + (b * 32 + n32) * KP + (2 * e + h) * 16);
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[e], s[b], 0, 0, 0);
+            }
+        }
+        float ks[NG], vs[NG], v_now = 0.0f;
+        int least = 0;// below 0: a group without a page
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            ks[g] = lane_of(here.k_scale, at + g);
+            vs[g] = lane_of(here.v_scale, at + g);
+            least |= __builtin_amdgcn_readlane(here.page, at + g);
+            v_now = fmaxf(v_now, vs[g]);
+        }
+        if (least < 0 || key0 + BK > all_see) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t key = key0 + b * 32 + 8 * (i / 4) + 4 * h + i % 4;
+                    const bool gone = key >= limit || __builtin_amdgcn_readlane(here.page, at + 2 * b + i / 8) < 0;
+                    s[b][i] = gone ? -__builtin_inff() : s[b][i];
+                }
+            }
+        }
+        if (v_now > 2.0f * v_top) {
+            const float next = fmaxf(v_now, 0x1p-100f), by = v_top / next;
+            v_top = next;
+            v_inv = 1.0f / next;
+#pragma unroll
+            for (int t = 0; t < TD; ++t) o[t] *= by;
+        }
+        float f[NG], high = kNone;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            // (above 0, so that what is not seen stays at minus infinity)
+            f[g] = fmaxf(factor * ks[g], 0x1p-126f);
+            const f32x16 &x = s[g / 2];
+            const int b = g % 2 * 8;
+            const float top = fmaxf(fmaxf(fmaxf(fmaxf(x[b], x[b + 1]), x[b + 2]), fmaxf(fmaxf(x[b + 3], x[b + 4]), x[b + 5])), fmaxf(x[b + 6], x[b + 7]));
+            high = fmaxf(high, top * f[g]);
+        }
+        if (__builtin_amdgcn_ballot_w64(high > m + (kLift + kSlack)) != 0) {
+            const float next = fmaxf(m, pair_max(high) - kLift), by = __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= by;
+#pragma unroll
+            for (int t = 0; t < TD; ++t) o[t] *= by;
+        }
+        f16x8 p[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const float ratio = fmaxf(vs[g] * v_inv, kLeastRatio), less = __builtin_amdgcn_logf(ratio) - m;
+            float y[8], sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + i], f[g], less));
+                sum += y[i];
+            }
+            l = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(ratio), l);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const f16x2 w = __builtin_convertvector((f32x2{y[i], y[i + 1]}), f16x2);
+                p[g][i] = w.x;
+                p[g][i + 1] = w.y;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+            for (int t = 0; t < TD; ++t) {
+                const f16x8 x = *reinterpret_cast<const f16x8 *>(v_lds[buffer] + (t * 32 + n32) * VP + g * 32 + h * 16);
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p[g], o[t], 0, 0, 0);
+            }
+        }
+    };
+
+    if (tiles != 0) {
+        load(0);
+        store(0);
+        if (tiles > 1) load(1);
+        __syncthreads();
+        for (uint32_t tile = 0; tile < tiles; ++tile) {
+            if (tile + 1 < tiles) store(tile + 1);
+            if (tile + 2 < tiles) load(tile + 2);
+            compute(tile);
+            __syncthreads();
+        }
+    }
+
+    if (!mine) return;
+    l += __shfl_xor(l, 32);// (the other half of a row is in the same wavefront, and stays or goes with it)
+    // o[t][i] is column TD m' + t of the row, m' = 8 (i / 4) + 4 h + i % 4
+    if (u.chunks > 1) {
+        const uint64_t at = (static_cast<uint64_t>(u.slot + u.chunk) * a.kv_heads + head) * a.tile_rows + wave * 32 + n32;
+        if (h == 0) {
+            a.part_stat[2 * at] = m;
+            a.part_stat[2 * at + 1] = l;
+        }
+        if (l == 0.0f) return;// not read
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float *p = a.part_out + at * DP + (8 * (i / 4) + 4 * h + i % 4) * TD;
+#pragma unroll
+            for (int t = 0; t < TD; t += 2) *reinterpret_cast<f32x2 *>(p + t) = f32x2{o[t][i] * v_top, o[t + 1][i] * v_top};
+        }
+    } else {
+        const float by = l > 0.0f ? v_top / l : 0.0f;
+        uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + q_head * a.out_head;
+        typedef uint32_t __attribute__((aligned(2))) u32_any;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t d = (8 * (i / 4) + 4 * h + i % 4) * TD;
+#pragma unroll
+            for (int t = 0; t < TD; t += 2) {
+                if (d + t < a.dim) *reinterpret_cast<u32_any *>(p + d + t) = narrow2_rne(a.bf16, o[t][i] * by, o[t + 1][i] * by);
+            }
+        }
+    }
+}
+
+template<bool FP8, int DP>
+void launch(const AttentionArgs &a, unsigned units, hipStream_t s) {
+    paged_attention_tiles<FP8, DP><<<units, paged_tile_waves(DP) * kWave, 0, s>>>(a);
+}
+template<bool FP8>
+void launch(const AttentionArgs &a, unsigned units, hipStream_t s) {
+    switch (paged_dim(a.dim)) {
+        case 64: return launch<FP8, 64>(a, units, s);
+        case 128: return launch<FP8, 128>(a, units, s);
+        case 192: return launch<FP8, 192>(a, units, s);
+        default: return launch<FP8, 256>(a, units, s);
+    }
+}
+
+}// namespace
+
+void amdLaunchPagedAttentionTiles(const AttentionArgs &a, bool fp8, unsigned units, hipStream_t s) { fp8 ? launch<true>(a, units, s) : launch<false>(a, units, s); }

@@ -25,7 +25,9 @@ struct AttentionArgs {
     FastDiv by_group, by_block, by_tile;
     float scale;// of the scores, times log2(e)
     float units_each;// 1 / target
-    uint32_t least_steps;// of a unit
+    uint32_t least_steps;// of a unit, and what their number is a multiple of
+    uint32_t whole_steps;
+    uint32_t least_rows, most_rows;// of a sequence that this kernel takes
     bool bf16;
     float *part_out, *part_stat;// [slot, kv head][tile row][padded dim], and [..][2]
 };
@@ -42,7 +44,9 @@ struct RowWork {
 };
 __device__ __forceinline__ RowWork row_work(const AttentionArgs &a, const RowSpan &s) {
     const uint32_t tokens = s.count < a.max_tokens ? s.count : a.max_tokens;
-    return RowWork{fast_quotient(tokens * a.group + a.tile_rows - 1, a.by_tile), (s.length + kStepKeys - 1) / kStepKeys};
+    const uint32_t rows = tokens * a.group;
+    if (rows < a.least_rows || rows > a.most_rows) return RowWork{0, 0};
+    return RowWork{fast_quotient(rows + a.tile_rows - 1, a.by_tile), (s.length + kStepKeys - 1) / kStepKeys};
 }
 
 // Unit number `index` of all (SPLIT: tile number `index` of those that have several units); false if there are fewer.
@@ -58,7 +62,8 @@ __device__ bool find_unit(const AttentionArgs &a, uint32_t index, uint64_t *slot
     block_scan64<WAVES>(work, slots, &total);
     // at least total / target, with room for the rounding of the product
     uint32_t steps = static_cast<uint32_t>(static_cast<float>(total) * a.units_each * 1.000001f) + 1;
-    steps = steps < a.least_steps ? a.least_steps : steps;
+    steps = steps < a.least_steps ? a.least_steps : steps > 0x40000000u ? 0x40000000u : steps;
+    steps = (steps + a.whole_steps - 1) & ~(a.whole_steps - 1);
     const auto chunks_of = [&](const RowWork &w) { return w.steps > steps ? (w.steps + steps - 1) / steps : 1u; };
     // low half: units (SPLIT: tiles of several), high half: slots of the workspace
     uint64_t mine = 0, all;
@@ -103,5 +108,8 @@ __device__ __forceinline__ uint32_t narrow2_rne(bool bf16, float a, float b) {
 }
 
 }// namespace amd
+
+// paged_attention_tiles.hip: many query rows
+void amdLaunchPagedAttentionTiles(const amd::AttentionArgs &a, bool fp8, unsigned units, hipStream_t s);
 
 #endif
