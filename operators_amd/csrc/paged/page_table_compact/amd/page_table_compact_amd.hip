@@ -3,8 +3,7 @@
 //     rank(p) = used pages below p
 //     p used, p >= used:  i = rank(p) - rank(used)        p free, p < used:  i = p - rank(p)
 // Three phases: (1) used pages marked and counted by chunk, (2) ranks, the pairs,
-// (3) table and counts.  Latency bound: a small table goes through the phases in
-// one workgroup and one launch.
+// (3) table and counts.  Latency bound, a launch for each phase.
 #include "../../page_table_kernel.h"
 #include "page_table_compact_amd.h"
 
@@ -12,7 +11,7 @@ namespace {
 
 using namespace amd;
 
-constexpr int kTableWaves = 4, kOneWaves = 16;
+constexpr int kTableWaves = 4;
 
 struct CompactArgs {
     const int *table, *lengths, *refcount;
@@ -100,27 +99,15 @@ __device__ void renumber(const CompactArgs &a, Crew crew) {
     }
 }
 
-__device__ __forceinline__ bool in_use(const CompactArgs &a, uint32_t p) { return a.refcount[p] > 0; }
-
 __global__ __launch_bounds__(kTableWaves *kWave) void page_table_used(CompactArgs a) {
     __shared__ uint32_t slots[kTableWaves];
-    mark_pages<kTableWaves>(Crew{blockIdx.x, gridDim.x}, a.pages, a.words, a.counts, slots, [&](uint32_t p) { return in_use(a, p); });
+    mark_pages<kTableWaves>(Crew{blockIdx.x, gridDim.x}, a.pages, a.words, a.counts, slots, [&](uint32_t p) { return a.refcount[p] > 0; });
 }
 __global__ __launch_bounds__(kTableWaves *kWave) void page_table_pairs(CompactArgs a) {
     __shared__ uint64_t slots[kTableWaves];
     pair_up<kTableWaves>(a, Crew{blockIdx.x, gridDim.x}, slots);
 }
 __global__ __launch_bounds__(kTableWaves *kWave) void page_table_renumber(CompactArgs a) { renumber<kTableWaves>(a, Crew{blockIdx.x, gridDim.x}); }
-__global__ __launch_bounds__(kOneWaves *kWave) void page_table_compact_one(CompactArgs a) {
-    __shared__ uint64_t slots[kOneWaves];
-    const Crew alone{0, 1};
-    mark_pages<kOneWaves>(alone, a.pages, a.words, a.counts, reinterpret_cast<uint32_t *>(slots), [&](uint32_t p) { return in_use(a, p); });
-    phase_end();
-    pair_up<kOneWaves>(a, alone, slots);
-    phase_end();
-    renumber<kOneWaves>(a, alone);
-}
-
 }// namespace
 
 infiniopStatus_t amdPageTableCompact(PageTableCompactAmdDescriptor_t desc, void *workspace, uint64_t workspace_size, void *new_table, void *new_refcount,
@@ -151,15 +138,11 @@ infiniopStatus_t amdPageTableCompact(PageTableCompactAmdDescriptor_t desc, void 
                         z.old_rows.stride, z.new_rows.stride, z.old_rows.rows, z.old_rows.cols, z.pages, z.page, d.pairs, amd::fast_div(z.page),
                         words, counts, counts + chunks};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (rows * z.old_rows.cols + z.pages <= 16384) {
-        page_table_compact_one<<<1, kOneWaves * amd::kWave, 0, s>>>(a);
-    } else {
-        const unsigned by_chunk = static_cast<unsigned>(chunks < 1024 ? chunks : 1024);
-        const uint64_t rest = rows > by_chunk ? rows : by_chunk;
-        page_table_used<<<by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
-        page_table_pairs<<<by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
-        page_table_renumber<<<static_cast<unsigned>(rest < 1024 ? rest : 1024), kTableWaves * amd::kWave, 0, s>>>(a);
-    }
+    const unsigned by_chunk = static_cast<unsigned>(chunks < 1024 ? chunks : 1024);
+    const uint64_t rest = rows > by_chunk ? rows : by_chunk;
+    page_table_used<<<by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
+    page_table_pairs<<<by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
+    page_table_renumber<<<static_cast<unsigned>(rest < 1024 ? rest : 1024), kTableWaves * amd::kWave, 0, s>>>(a);
     AMD_CHECK_HIP(hipGetLastError(), STATUS_EXECUTION_FAILED);
     return STATUS_SUCCESS;
 }

@@ -7,17 +7,10 @@
 
 namespace amd {
 
-// A phase of one of these operators is written for `count` workgroups of which
-// this is number `index`, so that it may be a launch of its own or a part of one.
+// The workgroups of a launch, and which of them this is.
 struct Crew {
     uint32_t index, count;
 };
-
-// What one phase wrote to memory, plainly or by atomics, to the next phase in the same workgroup.
-__device__ __forceinline__ void phase_end() {
-    __threadfence();
-    __syncthreads();
-}
 
 // The bits of `test(page)` for all pages of the crew's chunks, and how many are set in each chunk.
 template<int WAVES, typename F>

@@ -58,7 +58,7 @@ def run_compact(ctx, table, lengths, refs, page, room, in_place=False):
     return [x.cpu().tolist() for x in (nt, nc, pairs, result)]
 
 
-# the small tables go through one launch, the large ones through several
+# one chunk of pages and many, rows by the workgroup and by the lane
 SIZES = [(1, 1, 1, 1, 1), (1, 5, 9, 16, 4), (7, 6, 60, 16, 5), (64, 20, 1500, 3, 15), (300, 8, 2500, 16, 6), (513, 40, 20000, 64, 30), (5000, 9, 40000, 16, 6)]
 
 
