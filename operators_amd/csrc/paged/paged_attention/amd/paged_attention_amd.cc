@@ -9,9 +9,9 @@ namespace {
 constexpr uint32_t kFewRows = 32;
 
 // Only tiles of several units use the workspace: of those, a tile of k keys is cut at every c of them where the sum of
-// all k is at most target * c, so they are at most 2 target units of a head (ceil(x) <= 2 x from 1 on).
+// all k is at most (most_units - most_tiles) * c, so they are at most twice that many of a head (ceil(x) <= 2 x from 1 on).
 uint64_t workspace_of(const PagedAttentionShape &s, const amd::PagedCache &c) {
-    return s.most_tiles == 0 ? 0 : 2ull * s.target * c.kv_heads * s.tile_rows * (paged_dim(c.dim) + 2) * sizeof(float);
+    return s.most_tiles == 0 ? 0 : 2ull * (s.most_units - s.most_tiles) * c.kv_heads * s.tile_rows * (paged_dim(c.dim) + 2) * sizeof(float);
 }
 
 }// namespace
@@ -53,21 +53,27 @@ infiniopStatus_t amdCreatePagedAttentionDescriptor(AmdHandle_t handle, PagedAtte
 
     // a sequence with tokens has at most one tile that it does not fill
     const uint64_t busy = rows.rows < tokens ? rows.rows : tokens, query_rows = tokens * group, most_rows = max_tokens * group;
+    const uint64_t cus = static_cast<uint64_t>(handle->cu_count);
     PagedAttentionShape few{}, many{};
     // two sets of 16 rows share what they read; heads wider than 128 leave no registers for that
     few.tile_rows = most_rows <= 16 || cache.dim > 128 ? 16 : 32;
     few.least = 1;
     few.most = kFewRows;
-    few.most_tiles = static_cast<uint32_t>(query_rows / few.tile_rows + busy);
-    // about three workgroups of a unit for each of the compute units
-    few.target = static_cast<uint32_t>(amd::ceil_div(3ull * handle->cu_count, cache.kv_heads));
+    // (one sequence that may have many query rows goes to the kernel for prompts whatever it has: one launch less)
+    few.most_tiles = busy == 1 && most_rows > kFewRows ? 0 : static_cast<uint32_t>(query_rows / few.tile_rows + busy);
+    // as many units as the GPU holds, twice that where rows of unequal length meet (us, bf16, 64/8 heads x 128: 48 rows of
+    // 100 to 131072 tokens 389 and 353, 32 of 8192 95 and 96; one of 131072 53 and 56)
+    few.target = static_cast<uint32_t>(amd::ceil_div((rows.rows == 1 ? 2 : 4) * cus, cache.kv_heads));
+    few.most_units = few.target + few.most_tiles;
     many.tile_rows = 32 * paged_tile_waves(paged_dim(cache.dim));
-    many.least = kFewRows + 1;
+    many.least = busy == 1 ? 1 : kFewRows + 1;
     many.most = UINT32_MAX;
     many.most_tiles = most_rows <= kFewRows ? 0 : static_cast<uint32_t>(query_rows / many.tile_rows + busy);
-    many.target = static_cast<uint32_t>(amd::ceil_div(handle->cu_count, cache.kv_heads));
+    many.target = static_cast<uint32_t>(amd::ceil_div(cus, cache.kv_heads));// one workgroup fills a compute unit
+    many.at_once = rows.rows == 1 ? 0 : static_cast<uint32_t>(cus);
+    many.most_units = (rows.rows == 1 ? 1 : 3) * many.target + many.most_tiles;// (one row is cut evenly)
     for (const PagedAttentionShape &s : {few, many}) {
-        if ((static_cast<uint64_t>(s.target) + s.most_tiles) * cache.kv_heads > amd::max_grid_1d(512)) return STATUS_BAD_TENSOR_SHAPE;
+        if (static_cast<uint64_t>(s.most_units) * cache.kv_heads > amd::max_grid_1d(512)) return STATUS_BAD_TENSOR_SHAPE;
     }
     const uint64_t for_few = workspace_of(few, cache), for_many = workspace_of(many, cache), bytes = for_few > for_many ? for_few : for_many;
     auto *desc = new (std::nothrow) PagedAttentionAmdDescriptor{

@@ -11,14 +11,15 @@ constexpr int paged_tile_waves(int padded) { return padded <= 128 ? 8 : 4; }
 
 // How a call's work is cut up.  A tile is up to `tile_rows` query rows (token by
 // head of one K/V head's group) of one sequence; a unit is a tile over a range of
-// keys, and what one workgroup computes.  `target` units of a K/V head are aimed
-// at; a tile is split over several units where that gives fewer.  Sequences with
+// keys, and what one workgroup computes.  `target` units of a K/V head or up to three
+// times as many are aimed at; a tile is split over several where that gives fewer.  Sequences with
 // at least `least` and at most `most` query rows are taken, the others left to the
 // other kernel.
 struct PagedAttentionShape {
     uint32_t tile_rows;
     uint32_t most_tiles;// of one K/V head, whatever the offsets; 0: the kernel is not needed
-    uint32_t target;
+    uint32_t target, most_units;// most_units: of a head, whatever the lengths
+    uint32_t at_once;// workgroups that the GPU holds, if units are made to fit that; 0 if not
     uint32_t least, most;
 };
 

@@ -31,13 +31,11 @@ constexpr float kSlack = 4.0f;   // log2 by which a score may exceed the running
 constexpr float kNone = -1.0e30f;// the maximum of no score
 
 // maximum and sum over the four lanes that hold one query row
-__device__ __forceinline__ float quad_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
-}
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float quad_max(float v) { return across32(across16(v, larger), larger); }
 __device__ __forceinline__ float quad_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    const auto add = [](float a, float b) { return a + b; };
+    return across32(across16(v, add), add);
 }
 
 // What a lane reads of 32 keys: of K, 16 bytes of each 64 columns of keys (lane % 16) of either half; of V,
@@ -74,7 +72,7 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[WORDS
 }
 
 template<bool FP8, int DP, int NT>
-__global__ __launch_bounds__(kWaves *kWave) void paged_attention_rows(AttentionArgs a) {
+__global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <= 64 ? 4 : 3) - (NT - 1)) void paged_attention_rows(AttentionArgs a) {
     constexpr int KS = DP / 32, CH = DP / 64, VB = DP / 16, WORDS = DP / 64;
     __shared__ uint64_t slots[kWaves];
     __shared__ Unit shared_unit;
@@ -83,7 +81,7 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_rows(AttentionA
     Unit u;
     const uint32_t head = blockIdx.x % a.kv_heads;
     if (!find_unit<kWaves, false>(a, blockIdx.x / a.kv_heads, slots, &shared_unit, &u)) return;
-    const uint32_t lane = threadIdx.x & (kWave - 1), wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave)));
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tid / kWave)));
     const uint32_t n16 = lane & 15u, g = lane >> 4;
     const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens;
     const uint32_t row0 = u.tile * a.tile_rows, rows = tokens * a.group;
@@ -92,6 +90,39 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_rows(AttentionA
     const auto sees = [&](uint32_t token) { return static_cast<uint32_t>(seen + static_cast<int>(token) < 0 ? 0 : seen + static_cast<int>(token) + 1); };
     const uint32_t row_end = row0 + a.tile_rows < rows ? row0 + a.tile_rows : rows;
     const uint32_t all_see = sees(fast_quotient(row0, a.by_group)), some_see = sees(fast_quotient(row_end - 1, a.by_group));
+
+    // the lane's places within a page, relative to the half's first key
+    uint32_t k_off[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) k_off[c] = n16 * a.k_at.token + (c * 64 + g * 16 < a.dim ? c * 64 + g * 16 : 0);// (q is 0 behind dim)
+    const uint32_t v_off = g * 4 * a.v_at.token + (n16 * VB < a.dim ? n16 * VB : 0);                             // (not stored behind dim)
+    const uint8_t *k_base = a.k + static_cast<uint64_t>(head) * a.k_at.head, *v_base = a.v + static_cast<uint64_t>(head) * a.v_at.head;
+    const float *ks_base = a.k_scale + static_cast<int64_t>(head) * a.k_at.s_head, *vs_base = a.v_scale + static_cast<int64_t>(head) * a.v_at.s_head;
+    const int *table = a.rows.table + u.row * a.rows.stride;
+
+    const uint32_t end = (some_see + kStepKeys - 1) / kStepKeys;
+    const uint32_t s0 = u.chunk * u.steps, s1 = s0 + u.steps < end ? s0 + u.steps : end;
+    // steps s0 + wave, + 4, ...: page and scales of 32 of them are read at once, a half step by each lane;
+    // the first of these are on their way while the queries are made ready
+    int page = -1;
+    float k_scale = 0.0f, v_scale = 0.0f;
+    const auto groups = [&](uint32_t base) {
+        page = -1;
+        k_scale = v_scale = 0.0f;
+        const uint32_t key = ((base + kWaves * (lane >> 1)) * 2 + (lane & 1)) * 16;
+        if (key < u.length && base + kWaves * (lane >> 1) < s1) {
+            const uint32_t col = fast_quotient(key, a.rows.by_page);
+            page = table[col];
+            if (static_cast<uint32_t>(page) < a.pages) {
+                const uint32_t block = fast_quotient(key - col * a.rows.page, a.by_block);
+                k_scale = ks_base[page * a.k_at.s_page + block];
+                v_scale = vs_base[page * a.v_at.s_page + block];
+            } else {
+                page = -1;
+            }
+        }
+    };
+    groups(s0 + wave);
 
     // the query rows, as the second operand of S: lane's row, 8 columns of each step of 32
     f16x8 q[NT][KS];
@@ -143,53 +174,37 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_rows(AttentionA
     }
     float v_top = 0.0f, v_inv = 0.0f;// the largest V scale that O stands relative to, and its inverse
 
-    // the lane's places within a page, relative to the half's first key
-    uint32_t k_off[CH];
-#pragma unroll
-    for (int c = 0; c < CH; ++c) k_off[c] = n16 * a.k_at.token + (c * 64 + g * 16 < a.dim ? c * 64 + g * 16 : 0);// (q is 0 behind dim)
-    const uint32_t v_off = g * 4 * a.v_at.token + (n16 * VB < a.dim ? n16 * VB : 0);                             // (not stored behind dim)
-    const uint8_t *k_base = a.k + static_cast<uint64_t>(head) * a.k_at.head, *v_base = a.v + static_cast<uint64_t>(head) * a.v_at.head;
-    const float *ks_base = a.k_scale + static_cast<int64_t>(head) * a.k_at.s_head, *vs_base = a.v_scale + static_cast<int64_t>(head) * a.v_at.s_head;
-    const int *table = a.rows.table + u.row * a.rows.stride;
-
-    const uint32_t end = (some_see + kStepKeys - 1) / kStepKeys;
-    const uint32_t s0 = u.chunk * u.steps, s1 = s0 + u.steps < end ? s0 + u.steps : end;
-    // steps s0 + wave, + 4, ...: page, place in it and scales of 32 of them are read at once, a half step by each lane
     for (uint32_t base = s0 + wave; base < s1; base += kWaves * 32) {
-        int page = -1;
-        uint32_t place = 0;
-        float k_scale = 0.0f, v_scale = 0.0f;
-        {
-            const uint32_t key = ((base + kWaves * (lane >> 1)) * 2 + (lane & 1)) * 16;
-            if (key < u.length) {
-                const uint32_t col = fast_quotient(key, a.rows.by_page);
-                page = table[col];
-                place = key - col * a.rows.page;
-                if (static_cast<uint32_t>(page) < a.pages) {
-                    const uint32_t block = fast_quotient(place, a.by_block);
-                    k_scale = ks_base[page * a.k_at.s_page + block];
-                    v_scale = vs_base[page * a.v_at.s_page + block];
-                } else {
-                    page = -1;
-                }
-            }
-        }
+        if (base != s0 + wave) groups(base);
         const uint32_t count = (s1 - base + kWaves - 1) / kWaves < 32 ? (s1 - base + kWaves - 1) / kWaves : 32;
-        const auto load = [&](uint32_t i, Tile<DP> &t) {
+        // the next 32 keys' K is asked for before the scores of these are computed, their V after, in the place of this K
+        const auto of_half = [&](uint32_t i, int h, uint32_t *at) {
+            const uint32_t key = (base + kWaves * i) * kStepKeys + h * 16;
+            *at = key - fast_quotient(key, a.rows.by_page) * a.rows.page;
+            const int pg = __builtin_amdgcn_readlane(page, 2 * i + h);
+            return static_cast<int64_t>(pg < 0 ? 0 : pg);// (no page: any place will do, the keys are masked)
+        };
+        const auto load_k = [&](uint32_t i, Tile<DP> &t) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int pg = __builtin_amdgcn_readlane(page, 2 * i + h);
-                const uint32_t at = __builtin_amdgcn_readlane(place, 2 * i + h);
-                const int64_t there = pg < 0 ? 0 : pg;// (no page: any place will do, the keys are masked)
-                const uint8_t *kp = k_base + there * a.k_at.page + static_cast<uint64_t>(at) * a.k_at.token;
-                const uint8_t *vp = v_base + there * a.v_at.page + static_cast<uint64_t>(at) * a.v_at.token;
+                uint32_t at;
+                const int64_t pg = of_half(i, h, &at);
+                const uint8_t *p = k_base + pg * a.k_at.page + static_cast<uint64_t>(at) * a.k_at.token;
 #pragma unroll
-                for (int c = 0; c < CH; ++c) t.k[h][c] = ld16_stream(kp + k_off[c]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) load_words<WORDS>(vp + static_cast<uint64_t>(j) * a.v_at.token + v_off, t.v[h][j]);
+                for (int c = 0; c < CH; ++c) t.k[h][c] = ld16_stream(p + k_off[c]);
             }
         };
-        const auto step = [&](uint32_t i, Tile<DP> &t) {
+        const auto load_v = [&](uint32_t i, Tile<DP> &t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t at;
+                const int64_t pg = of_half(i, h, &at);
+                const uint8_t *p = v_base + pg * a.v_at.page + static_cast<uint64_t>(at) * a.v_at.token;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) load_words<WORDS>(p + static_cast<uint64_t>(j) * a.v_at.token + v_off, t.v[h][j]);
+            }
+        };
+        const auto step = [&](uint32_t i, Tile<DP> &t, Tile<DP> &next) {
             const uint32_t key0 = (base + kWaves * i) * kStepKeys;
             const int pg0 = __builtin_amdgcn_readlane(page, 2 * i), pg1 = __builtin_amdgcn_readlane(page, 2 * i + 1);
             const float ks[2] = {__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, k_scale), 2 * i)),
@@ -211,6 +226,7 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_rows(AttentionA
                     for (int t2 = 0; t2 < NT; ++t2) s[t2][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[t2][e], s[t2][h], 0, 0, 0);
                 }
             }
+            if (i + 1 < count) load_v(i + 1, next);
             const bool masked = pg0 < 0 || pg1 < 0 || key0 + kStepKeys > all_see;
             if (masked) {// also V's codes behind the row's end, which may be anything
 #pragma unroll
@@ -309,13 +325,14 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_rows(AttentionA
             }
         };
         Tile<DP> even, odd;
-        load(0, even);
+        load_k(0, even);
+        load_v(0, even);
         for (uint32_t i = 0; i < count; i += 2) {
-            if (i + 1 < count) load(i + 1, odd);
-            step(i, even);
+            if (i + 1 < count) load_k(i + 1, odd);
+            step(i, even, odd);
             if (i + 1 < count) {
-                if (i + 2 < count) load(i + 2, even);
-                step(i + 1, odd);
+                if (i + 2 < count) load_k(i + 2, even);
+                step(i + 1, odd, even);
             }
         }
     }
@@ -406,40 +423,71 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_rows(AttentionA
     }
 }
 
-// The units of a tile together: a wavefront takes one query row.
+// The units of a tile together: a wavefront takes one query row, or, where the tile has many units, the four of a
+// workgroup a quarter of a row's each (one sequence of 131072 keys in 64 units: 10.0 against 5.4 us).
 template<int DP>
 __global__ __launch_bounds__(kWaves *kWave) void paged_attention_join(AttentionArgs a) {
     constexpr int PER = DP / 64;
     __shared__ uint64_t slots[kWaves];
     __shared__ Unit shared_unit;
+    __shared__ float meet[kWaves][PER + 1][kWave];
     Unit u;
     const uint32_t head = blockIdx.x % a.kv_heads;
     if (!find_unit<kWaves, true>(a, blockIdx.x / a.kv_heads, slots, &shared_unit, &u)) return;
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave)));
     const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens, row0 = u.tile * a.tile_rows, left = tokens * a.group - row0;
     const uint32_t rows = left < a.tile_rows ? left : a.tile_rows;
-    for (uint32_t in_tile = blockIdx.y * kWaves + wave; in_tile < rows; in_tile += gridDim.y * kWaves) {
+    const bool four = u.chunks > 8;// wavefronts to a row
+    const uint32_t quarter = (u.chunks + kWaves - 1) / kWaves, c0 = four ? wave * quarter : 0, c1 = four && c0 + quarter < u.chunks ? c0 + quarter : u.chunks;
+    const uint32_t first = four ? blockIdx.y : blockIdx.y * kWaves + wave, step = four ? gridDim.y : gridDim.y * kWaves;
+    for (uint32_t in_tile = first; in_tile < rows; in_tile += step) {
         const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * a.tile_rows + in_tile; };
         float high = kNone;
         for (uint32_t c = lane; c < u.chunks; c += kWave) high = fmaxf(high, a.part_stat[2 * at(c)]);
         high = wave_max(high);
         float total = 0.0f, o[PER] = {};
-        for (uint32_t base = 0; base < u.chunks; base += kWave) {
+        for (uint32_t base = c0; base < c1; base += kWave) {
             const uint32_t mine = base + lane;
             float by = 0.0f, l = 0.0f;
-            if (mine < u.chunks) {
+            if (mine < c1) {
                 l = a.part_stat[2 * at(mine) + 1];
                 by = l > 0.0f ? __builtin_amdgcn_exp2f(a.part_stat[2 * at(mine)] - high) : 0.0f;
             }
             total += wave_sum(l * by);
-            const uint32_t n = u.chunks - base < kWave ? u.chunks - base : kWave;
-            for (uint32_t c = 0; c < n; ++c) {
-                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, by), c));
-                if (w == 0.0f) continue;// (a unit that saw nothing has written nothing)
-                const float *p = a.part_out + at(base + c) * DP + lane * PER;
+            const uint32_t n = c1 - base < kWave ? c1 - base : kWave;
+            // 16 loads under way at a time; a unit that saw nothing has written nothing, and what is read of it is not used
+            for (uint32_t k0 = 0; k0 < n; k0 += 16) {
+                float x[16][PER];
 #pragma unroll
-                for (int i = 0; i < PER; ++i) o[i] += w * p[i];
+                for (uint32_t k = 0; k < 16; ++k) {
+                    const float *p = a.part_out + at(base + (k0 + k < n ? k0 + k : n - 1)) * DP + lane * PER;
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) x[k][i] = p[i];
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < 16; ++k) {
+                    const float w = k0 + k < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, by), k0 + k)) : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) o[i] += w != 0.0f ? w * x[k][i] : 0.0f;
+                }
             }
+        }
+        if (four) {
+            meet[wave][PER][lane] = total;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) meet[wave][i][lane] = o[i];
+            __syncthreads();
+            total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) o[i] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                total += meet[w][PER][lane];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) o[i] += meet[w][i][lane];
+            }
+            __syncthreads();
+            if (wave != 0) continue;
         }
         const float by = total > 0.0f ? 1.0f / total : 0.0f;
         const uint32_t r = row0 + in_tile, token = fast_quotient(r, a.by_group);
@@ -458,13 +506,19 @@ void launch(const PagedAttentionAmdDescriptor &d, AttentionArgs a, hipStream_t s
         a.tile_rows = z.tile_rows;
         a.by_tile = fast_div(z.tile_rows);
         a.units_each = 1.0f / static_cast<float>(z.target);
+        a.rounds_each = z.at_once == 0 ? 0.0f : static_cast<float>(d.cache.kv_heads) / static_cast<float>(z.at_once);
         a.least_rows = z.least;
         a.most_rows = z.most;
         // the workspace: statistics of all slots, then their sums
-        a.part_out = a.part_stat + 4ull * z.target * d.cache.kv_heads * z.tile_rows;
-        return (z.target + z.most_tiles) * d.cache.kv_heads;
+        a.part_out = a.part_stat + 4ull * (z.most_units - z.most_tiles) * d.cache.kv_heads * z.tile_rows;
+        return z.most_units * d.cache.kv_heads;
     };
-    {
+    const auto join = [&](const PagedAttentionShape &z) {
+        // a tile of several units has two at least
+        const uint32_t cut = z.most_units - z.most_tiles, tiles = cut < z.most_tiles ? cut : z.most_tiles, rows = d.max_tokens * d.group;
+        paged_attention_join<DP><<<dim3(tiles * d.cache.kv_heads, rows < 8 ? rows : 8), kWaves * kWave, 0, s>>>(a);
+    };
+    if (d.few.most_tiles != 0) {
         const unsigned units = shape(d.few);
         a.least_steps = 8;
         a.whole_steps = 1;
@@ -474,15 +528,14 @@ void launch(const PagedAttentionAmdDescriptor &d, AttentionArgs a, hipStream_t s
         } else {
             paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
         }
-        // a tile of several units has two at least
-        paged_attention_join<DP><<<dim3(d.few.target * d.cache.kv_heads, d.few.tile_rows / kWaves), kWaves * kWave, 0, s>>>(a);
+        join(d.few);
     }
     if (d.many.most_tiles != 0) {
         const unsigned units = shape(d.many);
         a.least_steps = 16;
         a.whole_steps = 2;
         amdLaunchPagedAttentionTiles(a, FP8, units, s);
-        paged_attention_join<DP><<<dim3(d.many.target * d.cache.kv_heads, 8), kWaves * kWave, 0, s>>>(a);
+        join(d.many);
     }
 }
 

@@ -23,7 +23,9 @@ using namespace amd;
 constexpr float kLift = 10.0f, kSlack = 4.0f, kNone = -1.0e30f;// as in paged_attention_rows.hip
 constexpr float kLeastRatio = 0x1p-40f;// of a V scale to the largest: P times it is 0 in fp16
 
-__device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+__device__ __forceinline__ float pair_max(float v) {
+    return across32(v, [](float a, float b) { return fmaxf(a, b); });
+}
 
 template<bool FP8, int DP>
 __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_tiles(AttentionArgs a) {
@@ -320,7 +322,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     }
 
     if (!mine) return;
-    l += __shfl_xor(l, 32);// (the other half of a row is in the same wavefront, and stays or goes with it)
+    l = across32(l, [](float x, float y) { return x + y; });// (the other half of a row is in the same wavefront, and stays or goes with it)
     // o[t][i] is column TD m' + t of the row, m' = 8 (i / 4) + 4 h + i % 4
     if (u.chunks > 1) {
         const uint64_t at = (static_cast<uint64_t>(u.slot + u.chunk) * a.kv_heads + head) * a.tile_rows + wave * 32 + n32;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             a.part_stat[2 * at] = m;
             a.part_stat[2 * at + 1] = l;
         }
-        if (l == 0.0f) return;// not read
+        // (where l is 0 it is not read)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float *p = a.part_out + at * DP + (8 * (i / 4) + 4 * h + i % 4) * TD;

@@ -1,7 +1,7 @@
 // Which unit of a call's work a workgroup computes.  The lengths are known on the
 // GPU only, so every workgroup works it out for itself: the work of all rows is
 // added up, keys per unit follow from it, and the unit's place among those of all
-// rows gives the row.  One scan over the rows, a few hundred nanoseconds.
+// rows gives the row.  One scan over the rows, within a wavefront for up to 64.
 // Include from .hip files only.
 #ifndef INFINIOP_AMD_PAGED_ATTENTION_UNITS_H
 #define INFINIOP_AMD_PAGED_ATTENTION_UNITS_H
@@ -24,7 +24,7 @@ struct AttentionArgs {
     uint32_t pages, kv_heads, dim, group, max_tokens, tile_rows;
     FastDiv by_group, by_block, by_tile;
     float scale;// of the scores, times log2(e)
-    float units_each;// 1 / target
+    float units_each, rounds_each;// 1 / target; kv heads / workgroups at work at once, or 0
     uint32_t least_steps;// of a unit, and what their number is a multiple of
     uint32_t whole_steps;
     uint32_t least_rows, most_rows;// of a sequence that this kernel takes
@@ -49,10 +49,72 @@ __device__ __forceinline__ RowWork row_work(const AttentionArgs &a, const RowSpa
     return RowWork{fast_quotient(rows + a.tile_rows - 1, a.by_tile), (s.length + kStepKeys - 1) / kStepKeys};
 }
 
-// Unit number `index` of all (SPLIT: tile number `index` of those that have several units); false if there are fewer.
-template<int WAVES, bool SPLIT>
-__device__ bool find_unit(const AttentionArgs &a, uint32_t index, uint64_t *slots, Unit *shared, Unit *out) {
-    const uint32_t lanes = WAVES * kWave, run = (a.rows.rows + lanes - 1) / lanes, r0 = threadIdx.x * run;
+// How many units a row's tiles are cut into where a unit has up to `steps`.
+__device__ __forceinline__ uint32_t unit_chunks(const RowWork &w, uint32_t steps) { return w.steps > steps ? (w.steps + steps - 1) / steps : 1u; }
+
+// Steps of a unit, from the work of all rows.  Cut into `target` parts, rows of unequal length leave odd ends.  Where
+// many more workgroups wait than run (a.rounds_each is 0) these even out.  Otherwise the GPU takes the units in rounds,
+// and of target, 3/2, 2 and 3 times as many parts those are taken whose rounds are the shortest together (a unit's
+// beginning and end are worth 4 steps).  count(steps): units of all rows.
+template<typename F>
+__device__ __forceinline__ uint32_t unit_steps(const AttentionArgs &a, float total, F count) {
+    const auto cut = [&](float by) {
+        // at least total / target, with room for the roundings on the way
+        uint32_t steps = static_cast<uint32_t>(total * a.units_each * by * 1.00001f) + 1;
+        steps = steps < a.least_steps ? a.least_steps : steps > 0x40000000u ? 0x40000000u : steps;
+        return (steps + a.whole_steps - 1) & ~(a.whole_steps - 1);
+    };
+    uint32_t best = cut(1.0f);
+    if (a.rounds_each == 0.0f) return best;
+    float least = __builtin_inff();
+    uint32_t last = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t steps = cut(i == 0 ? 1.0f : i == 1 ? 2.0f / 3 : i == 2 ? 0.5f : 1.0f / 3);
+        if (steps == last) break;// (the least there may be)
+        last = steps;
+        const float time = ceilf(count(steps) * a.rounds_each) * static_cast<float>(steps + 4);
+        if (time < least) {
+            least = time;
+            best = steps;
+        }
+    }
+    return best;
+}
+
+// Unit `i` of the row (JOIN: tile `i`), whose tiles' units begin at slot `slot`.
+template<bool JOIN>
+__device__ __forceinline__ Unit unit_of(const AttentionArgs &a, uint32_t r, const RowSpan &s, const RowWork &w, uint32_t chunks, uint32_t i, uint32_t slot) {
+    const uint32_t nth = JOIN ? i : i / chunks;
+    // a prompt's last tiles see the most keys and begin first
+    return Unit{r, w.tiles - 1 - nth, JOIN ? 0 : i - nth * chunks, chunks, s.first, s.count, s.length,
+                ((w.steps + chunks - 1) / chunks + a.whole_steps - 1) & ~(a.whole_steps - 1), slot + nth * chunks};
+}
+
+// Unit number `index` of all (JOIN: tile number `index` of those that have several units); false if there are fewer.
+template<int WAVES, bool JOIN>
+__device__ __forceinline__ bool find_unit(const AttentionArgs &a, uint32_t index, uint64_t *slots, Unit *shared, Unit *out) {
+    const auto same = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); };
+    const uint32_t tid = threadIdx.x;
+    if (a.rows.rows <= kWave) {// a row for each lane: every wavefront finds it for itself, without a barrier
+        const uint32_t lane = tid & (kWave - 1);
+        RowSpan s{0, 0, 0};
+        if (lane < a.rows.rows) s = row_span(a.rows, lane);
+        const RowWork w = row_work(a, s);
+        const uint32_t steps = unit_steps(a, wave_sum(static_cast<float>(w.tiles) * static_cast<float>(w.steps)),
+                                          [&](uint32_t n) { return wave_sum(static_cast<float>(w.tiles * unit_chunks(w, n))); });
+        const uint32_t chunks = unit_chunks(w, steps), units = w.tiles * chunks, mine = JOIN ? (chunks > 1 ? w.tiles : 0) : units;
+        const uint32_t end = wave_scan(mine), in_slots = chunks > 1 ? units : 0, slot = wave_scan(in_slots) - in_slots;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(index < end && index >= end - mine);
+        if (hit == 0) return false;
+        const int l = __builtin_ctzll(hit);
+        const auto at = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l)); };
+        const RowSpan span{at(s.first), at(s.count), at(s.length)};
+        const RowWork work{at(w.tiles), at(w.steps)};
+        *out = unit_of<JOIN>(a, l, span, work, at(chunks), index - at(end - mine), at(slot));
+        return true;
+    }
+    const uint32_t lanes = WAVES * kWave, run = (a.rows.rows + lanes - 1) / lanes, r0 = tid * run;
     const uint32_t r1 = r0 + run < a.rows.rows ? r0 + run : a.rows.rows;
     uint64_t work = 0, total;
     for (uint32_t r = r0; r < r1; ++r) {
@@ -60,41 +122,41 @@ __device__ bool find_unit(const AttentionArgs &a, uint32_t index, uint64_t *slot
         work += static_cast<uint64_t>(w.tiles) * w.steps;
     }
     block_scan64<WAVES>(work, slots, &total);
-    // at least total / target, with room for the rounding of the product
-    uint32_t steps = static_cast<uint32_t>(static_cast<float>(total) * a.units_each * 1.000001f) + 1;
-    steps = steps < a.least_steps ? a.least_steps : steps > 0x40000000u ? 0x40000000u : steps;
-    steps = (steps + a.whole_steps - 1) & ~(a.whole_steps - 1);
-    const auto chunks_of = [&](const RowWork &w) { return w.steps > steps ? (w.steps + steps - 1) / steps : 1u; };
-    // low half: units (SPLIT: tiles of several), high half: slots of the workspace
+    const uint32_t steps = unit_steps(a, static_cast<float>(total), [&](uint32_t n) {
+        uint64_t units = 0, sum;
+        for (uint32_t r = r0; r < r1; ++r) {
+            const RowWork w = row_work(a, row_span(a.rows, r));
+            units += static_cast<uint64_t>(w.tiles) * unit_chunks(w, n);
+        }
+        block_scan64<WAVES>(units, slots, &sum);
+        return static_cast<float>(sum);
+    });
+    // low half: units (JOIN: tiles of several), high half: slots of the workspace
+    const auto counts = [&](const RowWork &w, uint32_t chunks) {
+        const uint64_t units = static_cast<uint64_t>(w.tiles) * chunks;
+        return (JOIN ? (chunks > 1 ? w.tiles : 0) : units) | (chunks > 1 ? units << 32 : 0);
+    };
     uint64_t mine = 0, all;
     for (uint32_t r = r0; r < r1; ++r) {
         const RowWork w = row_work(a, row_span(a.rows, r));
-        const uint32_t c = chunks_of(w);
-        const uint64_t units = static_cast<uint64_t>(w.tiles) * c;
-        mine += (SPLIT ? (c > 1 ? w.tiles : 0) : units) | (c > 1 ? units << 32 : 0);
+        mine += counts(w, unit_chunks(w, steps));
     }
     uint64_t before = block_scan64<WAVES>(mine, slots, &all);
-    if (index >= static_cast<uint32_t>(all)) return false;
+    if (index >= same(static_cast<uint32_t>(all))) return false;
     if (index >= static_cast<uint32_t>(before) && index < static_cast<uint32_t>(before + mine)) {
         for (uint32_t r = r0; r < r1; ++r) {
             const RowSpan s = row_span(a.rows, r);
             const RowWork w = row_work(a, s);
-            const uint32_t c = chunks_of(w);
-            const uint64_t units = static_cast<uint64_t>(w.tiles) * c;
-            const uint64_t n = (SPLIT ? (c > 1 ? w.tiles : 0) : units) | (c > 1 ? units << 32 : 0);
+            const uint32_t chunks = unit_chunks(w, steps);
+            const uint64_t n = counts(w, chunks);
             if (index < static_cast<uint32_t>(before + n)) {
-                const uint32_t i = index - static_cast<uint32_t>(before);
-                // a prompt's last tiles see the most keys and begin first
-                const uint32_t nth = SPLIT ? i : i / c;
-                *shared = Unit{r, w.tiles - 1 - nth, SPLIT ? 0 : i - nth * c, c, s.first, s.count, s.length, steps,
-                               static_cast<uint32_t>(before >> 32) + nth * c};
+                *shared = unit_of<JOIN>(a, r, s, w, chunks, index - static_cast<uint32_t>(before), static_cast<uint32_t>(before >> 32));
                 break;
             }
             before += n;
         }
     }
     __syncthreads();
-    const auto same = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); };
     *out = Unit{same(shared->row), same(shared->tile), same(shared->chunk), same(shared->chunks), same(shared->first),
                 same(shared->count), same(shared->length), same(shared->steps), same(shared->slot)};
     return true;

@@ -36,22 +36,44 @@ __device__ __forceinline__ RowSpan row_span(const RaggedRows &b, uint32_t r) {
     return RowSpan{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi - lo), static_cast<uint32_t>(len < 0 ? 0 : len > room ? room : len)};
 }
 
+// ---- within a wavefront, without LDS --------------------------------------------
+// Sum of this lane's value and all lower lanes'.
+template<int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v) {// 0 where there is none
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+template<int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t from_lane(uint64_t v) {
+    return from_lane<CTRL, ROWS>(static_cast<uint32_t>(v)) | static_cast<uint64_t>(from_lane<CTRL, ROWS>(static_cast<uint32_t>(v >> 32))) << 32;
+}
+template<typename U>
+__device__ __forceinline__ U wave_scan(U v) {
+    v += from_lane<0x111, 0xF>(v);       // row_shr:1
+    v += from_lane<0x112, 0xF>(v);       // row_shr:2
+    v += from_lane<0x114, 0xF>(v);       // row_shr:4
+    v += from_lane<0x118, 0xF>(v);       // row_shr:8
+    v += from_lane<0x142, 0xA>(v);       // row_bcast:15 -> rows 1, 3
+    return v + from_lane<0x143, 0xC>(v); // row_bcast:31 -> rows 2, 3
+}
+// Lanes 16 and 32 apart, by exchanging rows of 16 lanes between two copies.
+template<typename F>
+__device__ __forceinline__ float across16(float v, F both) {
+    const auto two = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return both(__uint_as_float(two[0]), __uint_as_float(two[1]));
+}
+template<typename F>
+__device__ __forceinline__ float across32(float v, F both) {
+    const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return both(__uint_as_float(two[0]), __uint_as_float(two[1]));
+}
+
 // ---- whole-number sums over a workgroup of WAVES wavefronts --------------------
 // slots: LDS, WAVES values; one use of it has to end with a barrier before the next begins.
-__device__ __forceinline__ uint64_t shuffle_up64(uint64_t v, int by) {
-    const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), by), hi = __shfl_up(static_cast<uint32_t>(v >> 32), by);
-    return lo | static_cast<uint64_t>(hi) << 32;
-}
 // The sum of the lower lanes' values (exclusive), and of all in `total`.
 template<int WAVES>
 __device__ __forceinline__ uint64_t block_scan64(uint64_t v, uint64_t *slots, uint64_t *total) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    uint64_t sum = v;
-#pragma unroll
-    for (int by = 1; by < kWave; by *= 2) {
-        const uint64_t other = shuffle_up64(sum, by);
-        if (lane >= by) sum += other;
-    }
+    const uint64_t sum = wave_scan(v);
     if (lane == kWave - 1) slots[wave] = sum;
     __syncthreads();
     uint64_t before = 0, all = 0;
