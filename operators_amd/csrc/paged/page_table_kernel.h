@@ -36,27 +36,6 @@ __device__ __forceinline__ void mark_pages(Crew crew, uint32_t pages, uint64_t *
     }
 }
 
-// The sum of counts[0 .. upto) and of counts[0 .. chunks), to every lane of the workgroup.
-template<int WAVES>
-__device__ __forceinline__ void count_before(const uint32_t *counts, uint32_t upto, uint32_t chunks, uint64_t *slots, uint32_t *before, uint32_t *all) {
-    uint64_t both = 0, total;// low half: all, high half: before
-    for (uint32_t c = threadIdx.x; c < chunks; c += WAVES * kWave) {
-        const uint64_t n = counts[c];
-        both += n | (c < upto ? n << 32 : 0);
-    }
-    block_scan64<WAVES>(both, slots, &total);
-    *all = static_cast<uint32_t>(total);
-    *before = static_cast<uint32_t>(total >> 32);
-}
-
-// How many bits of the chunk's words lie below bit `page` of it.
-__device__ __forceinline__ uint32_t bits_below(const uint64_t *words, uint32_t page) {
-    const uint32_t word = page / 64, first = page / kChunkPages * kChunkWords;
-    uint32_t n = 0;
-    for (uint32_t w = first; w < word; ++w) n += static_cast<uint32_t>(__builtin_popcountll(words[w]));
-    return n + static_cast<uint32_t>(__builtin_popcountll(words[word] & ((1ull << (page & 63)) - 1)));
-}
-
 }// namespace amd
 
 #endif

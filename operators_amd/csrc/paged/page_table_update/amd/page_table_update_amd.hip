@@ -5,9 +5,10 @@
 // Four phases, each of which needs all of the one before: (1) the rows that change
 // are laid aside, (2) counts, (3) free pages marked and counted, needs worked out,
 // rows written, (4) fresh pages handed out.  Whole numbers throughout, added by
-// atomics whose order does not matter.  Latency bound, a launch for each phase: a small
-// table in one workgroup of 1024 lanes measured 129 us (64 rows of 64, 4096 pages)
-// against 10 in four launches, one wait for memory after the other.
+// atomics whose order does not matter.  Latency bound.  A launch for each phase, or, where
+// the table fits the registers and the counts the LDS of one workgroup, all of them in
+// one launch with three waits for memory (64 rows of 64, 4096 pages: 15.3 us in four
+// launches, 8.6 in one).
 #include "../../page_table_kernel.h"
 #include "page_table_update_amd.h"
 
@@ -103,45 +104,56 @@ __device__ void work_out(const UpdateArgs &a, Crew crew, uint32_t *slots) {
 }
 
 // (4) fresh pages to the rows that grow.  ends: LDS, for each row the sum of the needs up to it and its own.
+// Everything that does not depend on something else is asked for at the start, and one scan adds up all of it.
 template<int WAVES>
 __device__ void hand_out(const UpdateArgs &a, Crew crew, uint32_t *ends, uint64_t *slots) {
-    const uint32_t lanes = WAVES * kWave, chunks = (a.pages + kChunkPages - 1) / kChunkPages;
+    const uint32_t lanes = WAVES * kWave, chunks = (a.pages + kChunkPages - 1) / kChunkPages, lane = threadIdx.x & (kWave - 1);
     const uint32_t run = (a.rows + lanes - 1) / lanes, r0 = threadIdx.x * run;
-    uint64_t mine = 0, total, wide = 0, all_wide;
+    // a chunk's words, one for each of 16 lanes of every wavefront
+    uint64_t words = lane < kChunkWords ? a.words[crew.index * kChunkWords + lane] : 0;
+    // free pages of the chunks before the first of this workgroup, and of all
+    uint64_t free = 0;
+    for (uint32_t c = threadIdx.x; c < chunks; c += lanes) {
+        const uint64_t n = a.counts[c];
+        free += n << 32 | (c < crew.index ? n : 0);
+    }
+    // low half: pages, high half: rows too wide
+    uint64_t mine = 0;
     for (uint32_t r = r0; r < r0 + run && r < a.rows; ++r) {
         const uint32_t n = a.need[r];
-        if (n == kTooWide) wide += 1;
-        else mine += n & ~kCopies;
+        mine += n == kTooWide ? 1ull << 40 : n & ~kCopies;
     }
+    uint64_t total, all;
     uint64_t at = block_scan64<WAVES>(mine, slots, &total);
-    block_scan64<WAVES>(wide, slots, &all_wide);
+    block_scan64<WAVES>(free, slots, &all);
     for (uint32_t r = r0; r < r0 + run && r < a.rows; ++r) {
         const uint32_t n = a.need[r];
         at += n == kTooWide ? 0 : n & ~kCopies;
         ends[r] = static_cast<uint32_t>(at);// (sums beyond 2^32 do not fit into the pages, and nothing is handed out)
     }
-    uint32_t unused, all_free;
-    count_before<WAVES>(a.counts, 0, chunks, slots, &unused, &all_free);
-    const bool fits = all_wide == 0 && total <= all_free;
-    __syncthreads();
+    const uint64_t wanted = total & ((1ull << 40) - 1), all_free = all >> 32;
+    const uint32_t wide = static_cast<uint32_t>(total >> 40);
+    const bool fits = wide == 0 && wanted <= all_free;
     for (uint32_t r = crew.index * lanes + threadIdx.x; r < a.rows; r += crew.count * lanes) {
         a.new_lengths[r] = static_cast<int>(a.before[r] + (fits && a.grow[r] > 0 ? a.grow[r] : 0));
     }
     if (crew.index == 0 && threadIdx.x == 0) {
-        const uint64_t lacks = total > all_free ? total - all_free : 0;
+        const uint64_t lacks = wanted > all_free ? wanted - all_free : 0;
         a.result[0] = lacks > 0x7FFFFFFF ? 0x7FFFFFFF : static_cast<int>(lacks);
-        a.result[1] = static_cast<int>(all_wide);
+        a.result[1] = static_cast<int>(wide);
     }
+    __syncthreads();
     if (!fits) return;// (uniform over the workgroup)
-    for (uint32_t c = crew.index; c < chunks; c += crew.count) {
-        uint32_t base;
-        count_before<WAVES>(a.counts, c, chunks, slots, &base, &unused);
-        if (base >= total) break;
-        for (uint32_t i = threadIdx.x; i < kChunkPages; i += lanes) {
-            const uint32_t p = c * kChunkPages + i;
-            if (((a.words[c * kChunkWords + i / 64] >> (i & 63)) & 1) == 0) continue;
-            const uint32_t k = base + bits_below(a.words, p);
-            if (k >= total) continue;
+    uint32_t base = static_cast<uint32_t>(all);
+    for (uint32_t c = crew.index; c < chunks && base < wanted;) {
+        // the free pages before each word of the chunk, and in all of it
+        const uint32_t bits = static_cast<uint32_t>(__builtin_popcountll(words)), upto = wave_scan(bits);
+        for (uint32_t w = threadIdx.x / kWave; w < kChunkWords; w += WAVES) {
+            const uint64_t word = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(words), w)) |
+                                  static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(words >> 32), w))) << 32;
+            const uint32_t p = c * kChunkPages + w * 64 + lane;
+            const uint32_t k = base + static_cast<uint32_t>(__builtin_amdgcn_readlane(upto - bits, w)) + static_cast<uint32_t>(__builtin_popcountll(word & ((1ull << lane) - 1)));
+            if (((word >> lane) & 1) == 0 || k >= wanted) continue;
             uint32_t lo = 0, hi = a.rows - 1;// the first row whose needs end beyond k
             while (lo < hi) {
                 const uint32_t mid = (lo + hi) / 2;
@@ -161,6 +173,13 @@ __device__ void hand_out(const UpdateArgs &a, Crew crew, uint32_t *ends, uint64_
                 row[has + nth - ((need & kCopies) != 0 ? 1 : 0)] = static_cast<int>(p);
             }
         }
+        // (more chunks than workgroups: pools of over a million pages)
+        const uint32_t next = c + crew.count;
+        if (next < chunks) {
+            for (uint32_t x = c; x < next; ++x) base += a.counts[x];
+            words = lane < kChunkWords ? a.words[next * kChunkWords + lane] : 0;
+        }
+        c = next;
     }
 }
 
@@ -175,6 +194,128 @@ __global__ __launch_bounds__(kTableWaves *kWave) void page_table_fresh(UpdateArg
     __shared__ uint64_t slots[kTableWaves];
     hand_out<kTableWaves>(a, Crew{blockIdx.x, gridDim.x}, ends, slots);
 }
+// All four phases in one workgroup of 1024 lanes: the table's entries in registers, 8 a lane at most, the counts in LDS.
+constexpr uint32_t kSmallLanes = 1024, kSmallEach = 8;
+constexpr uint32_t kSmallEntries = kSmallLanes * kSmallEach, kSmallPages = kSmallLanes * kSmallEach, kSmallRows = kSmallLanes;
+
+template<uint32_t EACH>// entries and pages of a lane
+__global__ __launch_bounds__(kSmallLanes) void page_table_update_small(UpdateArgs a, FastDiv by_cols) {
+    constexpr int WAVES = kSmallLanes / kWave;
+    __shared__ int refs[kSmallLanes * EACH];
+    __shared__ int source[kSmallRows], last[kSmallRows], grow[kSmallRows];
+    __shared__ uint32_t had[kSmallRows], before[kSmallRows], need[kSmallRows], ends[kSmallRows];// pages, tokens, growth
+    __shared__ uint64_t slots[WAVES];
+    const uint32_t tid = threadIdx.x;
+    if (tid < a.rows) {
+        const uint32_t s = static_cast<uint32_t>(a.source[tid]);
+        source[tid] = static_cast<int>(s);
+        grow[tid] = a.grow[tid];
+        had[tid] = pages_of(a, in_range(a, a.lengths[tid]));
+        before[tid] = s < a.rows ? in_range(a, a.lengths[s]) : 0;
+        last[tid] = -1;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) {
+        const uint32_t p = tid + i * kSmallLanes;
+        refs[p] = p < a.pages ? a.refcount[p] : 1;
+    }
+    __syncthreads();
+    int entry[EACH];
+    const auto in_row = [&](uint32_t i, uint32_t *r, uint32_t *c) {
+        const uint32_t e = tid + i * kSmallLanes;
+        *r = fast_quotient(e, by_cols);
+        *c = e - *r * a.cols;
+        return e < a.rows * a.cols;
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) {
+        uint32_t r, c;
+        entry[i] = -1;
+        if (!in_row(i, &r, &c)) continue;
+        const uint32_t s = static_cast<uint32_t>(source[r]), has = pages_of(a, before[r]);
+        const int own = a.table[r * a.stride + c];
+        entry[i] = s == r ? own : c < has ? a.table[s * a.stride + c] : -1;
+        if (s != r) {
+            if (c < had[r] && static_cast<uint32_t>(own) < a.pages) atomicAdd(refs + own, -1);
+            if (static_cast<uint32_t>(entry[i]) < a.pages) atomicAdd(refs + entry[i], 1);
+        }
+        if (c + 1 == has) last[r] = entry[i];
+    }
+    __syncthreads();
+    uint64_t wanted = 0, total;// low half: pages, high half: rows too wide
+    if (tid < a.rows) {
+        const uint32_t length = before[tid], has = pages_of(a, length), by = grow[tid] > 0 ? static_cast<uint32_t>(grow[tid]) : 0;
+        uint32_t n = kTooWide;
+        if (by <= a.cols * a.page - length) {
+            n = pages_of(a, length + by) - has;
+            const uint32_t p = static_cast<uint32_t>(last[tid]);
+            if (by != 0 && has * a.page != length && p < a.pages && refs[p] > 1) n = (n + 1) | kCopies;
+        }
+        need[tid] = n;
+        wanted = n == kTooWide ? 1ull << 32 : n & ~kCopies;
+        a.pairs[2 * tid] = -1;
+        a.pairs[2 * tid + 1] = -1;
+    }
+    const uint64_t end = block_scan64<WAVES>(wanted, slots, &total) + wanted;// (fewer than 2^25 pages are wanted by rows that are not too wide)
+    if (tid < a.rows) ends[tid] = static_cast<uint32_t>(end);
+    // a lane's pages are neighbours, for the order in which they are handed out
+    uint64_t mine = 0, all_free;
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) {
+        const uint32_t p = tid * EACH + i;
+        mine += p < a.pages && refs[p] == 0 ? 1 : 0;
+    }
+    uint32_t k = static_cast<uint32_t>(block_scan64<WAVES>(mine, slots, &all_free));
+    const uint32_t all = static_cast<uint32_t>(total), wide = static_cast<uint32_t>(total >> 32);
+    const bool fits = wide == 0 && all <= all_free;
+    uint32_t is_free = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) {
+        const uint32_t p = tid * EACH + i;
+        is_free |= p < a.pages && refs[p] == 0 ? 1u << i : 0;
+    }
+    if (tid < a.rows) a.new_lengths[tid] = static_cast<int>(before[tid] + (fits && grow[tid] > 0 ? grow[tid] : 0));
+    if (tid == 0) {
+        a.result[0] = all > all_free ? static_cast<int>(all - all_free) : 0;
+        a.result[1] = static_cast<int>(wide);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) {
+        uint32_t r, c;
+        if (in_row(i, &r, &c) && (source[r] != static_cast<int>(r) || a.new_table != a.table)) a.new_table[r * a.new_stride + c] = entry[i];
+    }
+    __syncthreads();// refs read, the table written
+    if (fits) {
+#pragma unroll 1
+        for (; is_free != 0 && k < all; is_free &= is_free - 1, ++k) {
+            const uint32_t p = tid * EACH + static_cast<uint32_t>(__builtin_ctz(is_free));
+            uint32_t lo = 0, hi = a.rows - 1;// the first row whose needs end beyond k
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (ends[mid] > k) hi = mid;
+                else lo = mid + 1;
+            }
+            const uint32_t n = need[lo], nth = k - (ends[lo] - (n & ~kCopies)), has = pages_of(a, before[lo]);
+            int *row = a.new_table + lo * a.new_stride;
+            refs[p] = 1;
+            if ((n & kCopies) != 0 && nth == 0) {
+                a.pairs[2 * lo] = last[lo];
+                a.pairs[2 * lo + 1] = static_cast<int>(p);
+                row[has - 1] = static_cast<int>(p);
+                atomicAdd(refs + last[lo], -1);
+            } else {
+                row[has + nth - ((n & kCopies) != 0 ? 1 : 0)] = static_cast<int>(p);
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) {
+        const uint32_t p = tid + i * kSmallLanes;
+        if (p < a.pages) a.new_refcount[p] = refs[p];
+    }
+}
+
 }// namespace
 
 infiniopStatus_t amdPageTableUpdate(PageTableUpdateAmdDescriptor_t desc, void *workspace, uint64_t workspace_size, void *new_table, void *new_lengths,
@@ -205,11 +346,19 @@ infiniopStatus_t amdPageTableUpdate(PageTableUpdateAmdDescriptor_t desc, void *w
                        z.old_rows.stride, z.new_rows.stride, z.old_rows.rows, z.old_rows.cols, z.pages, z.page, amd::fast_div(z.page),
                        words, counts, counts + chunks, counts + chunks + rows, reinterpret_cast<int *>(counts + chunks + 2 * rows)};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const unsigned by_row = static_cast<unsigned>(rows < 1024 ? rows : 1024), by_chunk = static_cast<unsigned>(chunks < 1024 ? chunks : 1024);
-    page_table_rows<<<by_row, kTableWaves * amd::kWave, 0, s>>>(a);
-    page_table_count<<<by_row, kTableWaves * amd::kWave, 0, s>>>(a);
-    page_table_needs<<<by_row > by_chunk ? by_row : by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
-    page_table_fresh<<<by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
+    const uint64_t entries = rows * z.old_rows.cols;
+    if (rows <= kSmallRows && entries <= kSmallEntries && z.pages <= kSmallPages) {
+        const amd::FastDiv by_cols = amd::fast_div(z.old_rows.cols);
+        const uint64_t most = entries > z.pages ? entries : z.pages;
+        if (most <= 4 * kSmallLanes) page_table_update_small<4><<<1, kSmallLanes, 0, s>>>(a, by_cols);
+        else page_table_update_small<kSmallEach><<<1, kSmallLanes, 0, s>>>(a, by_cols);
+    } else {
+        const unsigned by_row = static_cast<unsigned>(rows < 1024 ? rows : 1024), by_chunk = static_cast<unsigned>(chunks < 1024 ? chunks : 1024);
+        page_table_rows<<<by_row, kTableWaves * amd::kWave, 0, s>>>(a);
+        page_table_count<<<by_row, kTableWaves * amd::kWave, 0, s>>>(a);
+        page_table_needs<<<by_row > by_chunk ? by_row : by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
+        page_table_fresh<<<by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);
+    }
     AMD_CHECK_HIP(hipGetLastError(), STATUS_EXECUTION_FAILED);
     return STATUS_SUCCESS;
 }

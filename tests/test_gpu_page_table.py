@@ -58,8 +58,8 @@ def run_compact(ctx, table, lengths, refs, page, room, in_place=False):
     return [x.cpu().tolist() for x in (nt, nc, pairs, result)]
 
 
-# one chunk of pages and many, rows by the workgroup and by the lane
-SIZES = [(1, 1, 1, 1, 1), (1, 5, 9, 16, 4), (7, 6, 60, 16, 5), (64, 20, 1500, 3, 15), (300, 8, 2500, 16, 6), (513, 40, 20000, 64, 30), (5000, 9, 40000, 16, 6)]
+# one workgroup with 4 and with 8 entries a lane, and several launches
+SIZES = [(1, 1, 1, 1, 1), (1, 5, 9, 16, 4), (7, 6, 60, 16, 5), (64, 20, 1500, 3, 15), (300, 8, 2500, 16, 6), (200, 30, 6000, 16, 20), (513, 40, 20000, 64, 30), (5000, 9, 40000, 16, 6)]
 
 
 @pytest.mark.parametrize("in_place", [False, True])
@@ -122,13 +122,46 @@ def test_compact(ctx, rows, cols, pages, page, most, in_place):
             assert again[0] == want[0] and again[1] == want[1] and again[3][1] == 0
 
 
-@pytest.mark.parametrize("pages", [1, 2, 63, 64, 65, 1023, 1024, 1025, 20000])
+@pytest.mark.parametrize("pages", [1, 2, 63, 64, 65, 1023, 1024, 1025, 8192, 8193, 9216, 20000])
 def test_compact_edges(ctx, pages):
     room = pages // 2
     for refs in ([0] * pages, [1] * pages, [0] * (pages // 2) + [2] * (pages - pages // 2), [1] * (pages // 2) + [0] * (pages - pages // 2),
                  [p % 2 for p in range(pages)], [0] * (pages - 1) + [5]):
         table, lengths = [[p, pages + 5, -1] for p in range(min(pages, 40))], [3] * min(pages, 40)
         assert run_compact(ctx, table, lengths, refs, 2, room) == list(ref.compact(table, lengths, refs, 2, room))
+
+
+def test_pools_of_more_chunks_than_workgroups(ctx):
+    """1.3 million pages: a workgroup goes through several chunks of 1024."""
+    pages, page, rows, cols = 1300000, 16, 40, 400
+    g = torch.Generator().manual_seed(9)
+    refs = (torch.rand(pages, generator=g) < 0.6).int()
+    refs[100000:1200000] = 1  # the free ones are far apart
+    free = (refs == 0).nonzero().flatten()
+    table, lengths = torch.full((rows, cols), -1, dtype=torch.int32), torch.zeros(rows, dtype=torch.int32)
+    high = (refs[1250000:] > 0).nonzero().flatten()[:rows * 3].view(rows, 3) + 1250000
+    table[:, :3], lengths[:] = high.int(), 3 * page
+    grow = 390 * page  # 15600 fresh pages
+    assert rows * 390 <= len(free)
+    t, n, c, result = table.to(DEV), lengths.to(DEV), refs.to(DEV), ints([9, 9])
+    pairs = torch.empty(rows, 2, dtype=torch.int32, device=DEV)
+    ctx.page_table_update(t, n, c, pairs, result, t, n, c, ints(list(range(rows))), ints([grow] * rows), page)
+    assert result.tolist() == [0, 0] and (pairs == -1).all() and (n == 393 * page).all()
+    want = table.clone()
+    want[:, 3:393] = free[:rows * 390].view(rows, 390).int()
+    assert torch.equal(t.cpu(), want)
+    refs[free[:rows * 390]] = 1
+    assert torch.equal(c.cpu(), refs)
+    moves = torch.empty(pages // 2, 2, dtype=torch.int32, device=DEV)
+    ctx.page_table_compact(t, c, moves, result, t, n, c, page)
+    used = int((refs > 0).sum())
+    above, below = (refs[used:] > 0).nonzero().flatten() + used, (refs[:used] == 0).nonzero().flatten()
+    assert result.tolist() == [used, len(above)] and len(above) == len(below)
+    assert torch.equal(moves[:len(above)].cpu(), torch.stack([above, below], 1).int()) and (moves[len(above):] == -1).all()
+    goes = torch.arange(pages)
+    goes[above] = below
+    assert torch.equal(t.cpu(), torch.where(want >= 0, goes[want.clamp(min=0).long()].int(), want))
+    assert (c[:used] == 1).all() and (c[used:] == 0).all()
 
 
 def test_captured_update_and_compact(ctx):
