@@ -21,7 +21,7 @@ namespace {
 using namespace amd;
 
 constexpr float kLift = 10.0f, kSlack = 4.0f, kNone = -1.0e30f;// as in paged_attention_rows.hip
-constexpr float kLeastRatio = 0x1p-40f;// of a V scale to the largest: P times it is 0 in fp16
+constexpr float kLeastRatio = -40.0f;// log2 of a V scale to the largest: P times it is 0 in fp16
 
 __device__ __forceinline__ float pair_max(float v) {
     return across32(v, [](float a, float b) { return fmaxf(a, b); });
@@ -98,7 +98,8 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
     }
-    float m = kNone, l = 0.0f, v_top = 0.0f, v_inv = 0.0f;
+    // the running maximum less 10, its sum, and log2 of the largest V scale so far, which O stands relative to
+    float m = kNone, l = 0.0f, v_top = kNone;
 
     // a lane's pieces of a tile: 16 bytes of one key of K, 4 bytes of 4 keys of V
     const auto k_key = [&](int i) { return (tid + i * kLanes) / NC; };
@@ -106,6 +107,9 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     const auto v_keys = [&](int i) { return (tid + i * kLanes) / (DP / 4) * 4; };
     const auto v_col = [&](int i) { return (tid + i * kLanes) % (DP / 4) * 4; };
     const auto works = [&](int i) { return K_TASKS % kLanes == 0 || tid + i * kLanes < K_TASKS; };
+    // (the 16 keys it is of: the same for the whole wavefront, for 16 keys are the pieces of whole wavefronts, or a
+    // wavefront's pieces lie within 16 keys)
+    const auto group_of = [](uint32_t key) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(key / 16))); };
     uint32_t k_off[PER], v_off[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -119,81 +123,89 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     const uint32_t end = (tile_sees + kStepKeys - 1) / kStepKeys;
     const uint32_t s0 = u.chunk * u.steps, s1 = s0 + u.steps < end ? s0 + u.steps : end;
     const uint32_t first_key = s0 * kStepKeys, tiles = s1 > s0 ? (s1 - s0 + NB - 1) / NB : 0;
+    const uint32_t my_tiles = some_see <= first_key ? 0 : (some_see - first_key + BK - 1) / BK < tiles ? (some_see - first_key + BK - 1) / BK : tiles;
 
-    // pages, places in them and scales of 64 groups of 16 keys, one for each lane: those of the tiles that are computed
-    // with, and those of the tiles that are loaded (which run ahead)
+    // What a tile is loaded and computed with is read for 64 groups of 16 keys at once, one for each lane: their pages
+    // for K and for V, which are loaded three and two tiles ahead, and pages and scales for the computation.
     constexpr uint32_t kAhead = 64 / NG;// tiles of such a set
-    struct Groups {
-        int page;
-        uint32_t place;
-        float k_scale, v_scale;
-    };
-    const auto groups_of = [&](uint32_t tile) {
-        Groups g{-1, 0, 0.0f, 0.0f};
+    const auto page_of = [&](uint32_t tile) {
         const uint32_t key = first_key + tile * BK + lane * 16;
-        if (key < u.length) {
-            const uint32_t col = fast_quotient(key, a.rows.by_page);
-            g.page = table[col];
-            g.place = key - col * a.rows.page;
-            if (static_cast<uint32_t>(g.page) < a.pages) {
-                const uint32_t block = fast_quotient(g.place, a.by_block);
-                g.k_scale = ks_base[g.page * a.k_at.s_page + block];
-                g.v_scale = vs_base[g.page * a.v_at.s_page + block];
-            } else {
-                g.page = -1;
-            }
+        if (key >= u.length) return -1;
+        const int page = table[fast_quotient(key, a.rows.by_page)];
+        return static_cast<uint32_t>(page) < a.pages ? page : -1;
+    };
+    const auto place_of = [&](uint32_t key) { return key - fast_quotient(key, a.rows.by_page) * a.rows.page; };
+    int k_pages = -1, v_pages = -1, page = -1;
+    float k_scale = 0.0f, v_log = kNone;
+    const auto scales = [&](uint32_t tile) {
+        page = page_of(tile);
+        k_scale = 0.0f;
+        v_log = -200.0f;
+        if (page >= 0) {
+            const uint32_t block = fast_quotient(place_of(first_key + tile * BK + lane * 16), a.by_block);
+            k_scale = ks_base[page * a.k_at.s_page + block];
+            v_log = __builtin_amdgcn_logf(fmaxf(vs_base[page * a.v_at.s_page + block], 0x1p-126f));
         }
-        return g;
     };
     const auto lane_of = [](float v, uint32_t l2) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l2)); };
 
     u32x4 k_raw[PER];
     uint32_t v_raw[PER][4];
     int v_live[PER];// how many of the 4 keys there are
-    Groups ahead = groups_of(0), here = ahead;
-    const auto load = [&](uint32_t tile) {
-        if (tile % kAhead == 0 && tile != 0) ahead = groups_of(tile);
-        const uint32_t at = tile % kAhead * NG;
+    const auto load_k = [&](uint32_t tile) {
+        if (tile % kAhead == 0) k_pages = page_of(tile);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (!works(i)) continue;
-            // (the same group for the whole wavefront: 16 keys are the pieces of whole wavefronts, or a wavefront's are within 16 keys)
-            const uint32_t kg = at + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(k_key(i) / 16)));
-            const uint32_t vg = at + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v_keys(i) / 16)));
-            const int kp = __builtin_amdgcn_readlane(ahead.page, kg), vp = __builtin_amdgcn_readlane(ahead.page, vg);
-            const uint32_t k_place = __builtin_amdgcn_readlane(ahead.place, kg), v_place = __builtin_amdgcn_readlane(ahead.place, vg);
-            const uint8_t *k = k_base + static_cast<int64_t>(kp < 0 ? 0 : kp) * a.k_at.page + static_cast<uint64_t>(k_place) * a.k_at.token;
-            const uint8_t *v = v_base + static_cast<int64_t>(vp < 0 ? 0 : vp) * a.v_at.page + static_cast<uint64_t>(v_place) * a.v_at.token;
-            k_raw[i] = ld16(k + k_off[i]);
-            v_live[i] = vp < 0 ? 0 : static_cast<int>(u.length) - static_cast<int>(first_key + tile * BK + v_keys(i));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v_raw[i][j] = *reinterpret_cast<const uint32_t *>(v + static_cast<uint64_t>(j) * a.v_at.token + v_off[i]);
+            const uint32_t g = group_of(k_key(i));
+            const int pg = __builtin_amdgcn_readlane(k_pages, tile % kAhead * NG + g);
+            k_raw[i] = ld16(k_base + static_cast<int64_t>(pg < 0 ? 0 : pg) * a.k_at.page +
+                            static_cast<uint64_t>(place_of(first_key + tile * BK + g * 16)) * a.k_at.token + k_off[i]);
         }
     };
-    const auto store = [&](uint32_t tile) {
-        const uint32_t buffer = tile & 1u;
+    const auto load_v = [&](uint32_t tile) {
+        if (tile % kAhead == 0) v_pages = page_of(tile);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (!works(i)) continue;
-            uint8_t *k = k_lds[buffer] + k_key(i) * KP + k_piece(i) * 16;
-            f16x8 lo, hi;
+            const uint32_t g = group_of(v_keys(i));
+            const int pg = __builtin_amdgcn_readlane(v_pages, tile % kAhead * NG + g);
+            const uint8_t *p = v_base + static_cast<int64_t>(pg < 0 ? 0 : pg) * a.v_at.page +
+                               static_cast<uint64_t>(place_of(first_key + tile * BK + g * 16)) * a.v_at.token;
+            v_live[i] = pg < 0 ? 0 : static_cast<int>(u.length) - static_cast<int>(first_key + tile * BK + v_keys(i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v_raw[i][j] = *reinterpret_cast<const uint32_t *>(p + static_cast<uint64_t>(j) * a.v_at.token + v_off[i]);
+        }
+    };
+    const auto store_k = [&](uint32_t tile) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (!works(i)) continue;
+            uint8_t *k = k_lds[tile & 1u] + k_key(i) * KP + k_piece(i) * 16;
+            f16x8 half[2];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const uint32_t c = prepare_codes<FP8>(k_raw[i][w]);
                 const f16x2 x = pair_of<FP8, false>(c), y = pair_of<FP8, true>(c);
-                f16x8 &to = w < 2 ? lo : hi;
+                f16x8 &to = half[w / 2];
                 to[w % 2 * 4] = x.x;
                 to[w % 2 * 4 + 1] = x.y;
                 to[w % 2 * 4 + 2] = y.x;
                 to[w % 2 * 4 + 3] = y.y;
             }
-            *reinterpret_cast<f16x8 *>(k) = lo;
-            *reinterpret_cast<f16x8 *>(k + NC * 16) = hi;
+            *reinterpret_cast<f16x8 *>(k) = half[0];
+            *reinterpret_cast<f16x8 *>(k + NC * 16) = half[1];
+        }
+    };
+    const auto store_v = [&](uint32_t tile) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (!works(i)) continue;
             uint32_t x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = v_raw[i][j];
             // what lies behind the row's end, or in no page, may be anything: no number times 0 is 0
-            if (v_live[i] < 4) {
+            if (__builtin_amdgcn_ballot_w64(v_live[i] < 4) != 0) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = j >= v_live[i] ? 0 : x[j];
             }
@@ -212,38 +224,52 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
                 const auto two = [&](int j) { return __builtin_bit_cast(uint32_t, c % 2 ? pair_of<FP8, true>(pair[j][c / 2]) : pair_of<FP8, false>(pair[j][c / 2])); };
                 // column d is row d / TD of the accumulator's tile d % TD
                 const uint32_t d = v_col(i) + c, row = d % TD * 32 + d / TD;
-                *reinterpret_cast<u32x2 *>(v_lds[buffer] + row * VP + place * 2) = u32x2{two(0), two(1)};
+                *reinterpret_cast<u32x2 *>(v_lds[tile & 1u] + row * VP + place * 2) = u32x2{two(0), two(1)};
             }
         }
     };
 
-    const auto compute = [&](uint32_t tile) {
-        const uint32_t key0 = first_key + tile * BK, buffer = tile & 1u;
-        if (tile % kAhead == 0 && tile != 0) here = groups_of(tile);
-        if (key0 >= some_see) return;
-        const uint32_t at = tile % kAhead * NG;
-        f32x16 s[NB];
+    // The scores of a tile as the matrix units leave them, and what they are multiplied by.
+    f32x16 s[NB];
+    float f[NG], high = kNone;
+    const auto products = [&](uint32_t tile, f32x16(&x)[NB]) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) x[b][i] = 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < KS; ++e) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const f16x8 x = *reinterpret_cast<const f16x8 *>(k_lds[buffer] + (b * 32 + n32) * KP + (2 * e + h) * 16);
-                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[e], s[b], 0, 0, 0);
+                const f16x8 k = *reinterpret_cast<const f16x8 *>(k_lds[tile & 1u] + (b * 32 + n32) * KP + (2 * e + h) * 16);
+                x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], x[b], 0, 0, 0);
             }
         }
-        float ks[NG], vs[NG], v_now = 0.0f;
+    };
+    // The largest score, from the largest product of each group.
+    const auto largest = [&](uint32_t tile) {
+        const uint32_t at = tile % kAhead * NG;
+        high = kNone;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            // (above 0, so that what is not seen stays at minus infinity)
+            f[g] = fmaxf(factor * lane_of(k_scale, at + g), 0x1p-126f);
+            const f32x16 &x = s[g / 2];
+            const int b = g % 2 * 8;
+            const float top = fmaxf(fmaxf(fmaxf(fmaxf(x[b], x[b + 1]), x[b + 2]), fmaxf(fmaxf(x[b + 3], x[b + 4]), x[b + 5])), fmaxf(x[b + 6], x[b + 7]));
+            high = fmaxf(high, top * f[g]);
+        }
+    };
+    // What a tile's scores need before their exponentials: its scales, the mask, the maximum, the V scale.
+    const auto ready = [&](uint32_t tile) {
+        const uint32_t key0 = first_key + tile * BK, at = tile % kAhead * NG;
+        float v_now = kNone;
         int least = 0;// below 0: a group without a page
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            ks[g] = lane_of(here.k_scale, at + g);
-            vs[g] = lane_of(here.v_scale, at + g);
-            least |= __builtin_amdgcn_readlane(here.page, at + g);
-            v_now = fmaxf(v_now, vs[g]);
+            least |= __builtin_amdgcn_readlane(page, at + g);
+            v_now = fmaxf(v_now, lane_of(v_log, at + g));
         }
         if (least < 0 || key0 + BK > all_see) {
 #pragma unroll
@@ -251,27 +277,17 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const uint32_t key = key0 + b * 32 + 8 * (i / 4) + 4 * h + i % 4;
-                    const bool gone = key >= limit || __builtin_amdgcn_readlane(here.page, at + 2 * b + i / 8) < 0;
+                    const bool gone = (key >= limit) | (__builtin_amdgcn_readlane(page, at + 2 * b + i / 8) < 0);
                     s[b][i] = gone ? -__builtin_inff() : s[b][i];
                 }
             }
+            largest(tile);
         }
-        if (v_now > 2.0f * v_top) {
-            const float next = fmaxf(v_now, 0x1p-100f), by = v_top / next;
-            v_top = next;
-            v_inv = 1.0f / next;
+        if (v_now > v_top + 1.0f) {
+            const float by = __builtin_amdgcn_exp2f(v_top - v_now);
+            v_top = v_now;
 #pragma unroll
             for (int t = 0; t < TD; ++t) o[t] *= by;
-        }
-        float f[NG], high = kNone;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            // (above 0, so that what is not seen stays at minus infinity)
-            f[g] = fmaxf(factor * ks[g], 0x1p-126f);
-            const f32x16 &x = s[g / 2];
-            const int b = g % 2 * 8;
-            const float top = fmaxf(fmaxf(fmaxf(fmaxf(x[b], x[b + 1]), x[b + 2]), fmaxf(fmaxf(x[b + 3], x[b + 4]), x[b + 5])), fmaxf(x[b + 6], x[b + 7]));
-            high = fmaxf(high, top * f[g]);
         }
         if (__builtin_amdgcn_ballot_w64(high > m + (kLift + kSlack)) != 0) {
             const float next = fmaxf(m, pair_max(high) - kLift), by = __builtin_amdgcn_exp2f(m - next);
@@ -280,46 +296,73 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
 #pragma unroll
             for (int t = 0; t < TD; ++t) o[t] *= by;
         }
-        f16x8 p[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const float ratio = fmaxf(vs[g] * v_inv, kLeastRatio), less = __builtin_amdgcn_logf(ratio) - m;
-            float y[8], sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + i], f[g], less));
-                sum += y[i];
-            }
-            l = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(ratio), l);
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const f16x2 w = __builtin_convertvector((f32x2{y[i], y[i + 1]}), f16x2);
-                p[g][i] = w.x;
-                p[g][i + 1] = w.y;
-            }
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-#pragma unroll
-            for (int t = 0; t < TD; ++t) {
-                const f16x8 x = *reinterpret_cast<const f16x8 *>(v_lds[buffer] + (t * 32 + n32) * VP + g * 32 + h * 16);
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p[g], o[t], 0, 0, 0);
-            }
-        }
     };
 
     if (tiles != 0) {
-        load(0);
-        store(0);
-        if (tiles > 1) load(1);
+        load_k(0);
+        store_k(0);
+        load_v(0);
+        if (tiles > 1) {
+            load_k(1);
+            store_k(1);
+        }
+        store_v(0);
+        if (tiles > 2) load_k(2);
+        if (tiles > 1) load_v(1);
+        scales(0);
+        __syncthreads();
+        if (my_tiles != 0) {
+            products(0, s);
+            largest(0);
+            ready(0);
+        }
         __syncthreads();
         for (uint32_t tile = 0; tile < tiles; ++tile) {
-            if (tile + 1 < tiles) store(tile + 1);
-            if (tile + 2 < tiles) load(tile + 2);
-            compute(tile);
+            if (tile + 2 < tiles) store_k(tile + 2);
+            if (tile + 1 < tiles) store_v(tile + 1);
+            if (tile + 3 < tiles) load_k(tile + 3);
+            if (tile + 2 < tiles) load_v(tile + 2);
+            if (tile < my_tiles) {
+                const uint32_t at = tile % kAhead * NG;
+                f16x8 p[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const float v = fmaxf(lane_of(v_log, at + g) - v_top, kLeastRatio), less = v - m;
+                    float y[8], sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + i], f[g], less));
+                        sum += y[i];
+                    }
+                    l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-v), l);
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const f16x2 w = __builtin_convertvector((f32x2{y[i], y[i + 1]}), f16x2);
+                        p[g][i] = w.x;
+                        p[g][i + 1] = w.y;
+                    }
+                }
+                if ((tile + 1) % kAhead == 0) scales(tile + 1);
+                // the next tile's products, beside this one's exponentials (behind the last they are not used)
+                f32x16 next[NB];
+                products(tile + 1, next);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+#pragma unroll
+                    for (int t = 0; t < TD; ++t) {
+                        const f16x8 x = *reinterpret_cast<const f16x8 *>(v_lds[tile & 1u] + (t * 32 + n32) * VP + g * 32 + h * 16);
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p[g], o[t], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) s[b] = next[b];
+                largest(tile + 1);
+                if (tile + 1 < my_tiles) ready(tile + 1);
+            }
             __syncthreads();
         }
     }
+    const float v_unit = __builtin_amdgcn_exp2f(fmaxf(v_top, -140.0f));
 
     if (!mine) return;
     l = across32(l, [](float x, float y) { return x + y; });// (the other half of a row is in the same wavefront, and stays or goes with it)
@@ -335,10 +378,10 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         for (int i = 0; i < 16; ++i) {
             float *p = a.part_out + at * DP + (8 * (i / 4) + 4 * h + i % 4) * TD;
 #pragma unroll
-            for (int t = 0; t < TD; t += 2) *reinterpret_cast<f32x2 *>(p + t) = f32x2{o[t][i] * v_top, o[t + 1][i] * v_top};
+            for (int t = 0; t < TD; t += 2) *reinterpret_cast<f32x2 *>(p + t) = f32x2{o[t][i] * v_unit, o[t + 1][i] * v_unit};
         }
     } else {
-        const float by = l > 0.0f ? v_top / l : 0.0f;
+        const float by = l > 0.0f ? v_unit / l : 0.0f;
         uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + q_head * a.out_head;
         typedef uint32_t __attribute__((aligned(2))) u32_any;
 #pragma unroll
