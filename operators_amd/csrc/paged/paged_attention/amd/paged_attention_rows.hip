@@ -513,10 +513,10 @@ void launch(const PagedAttentionAmdDescriptor &d, AttentionArgs a, hipStream_t s
         a.part_out = a.part_stat + 4ull * (z.most_units - z.most_tiles) * d.cache.kv_heads * z.tile_rows;
         return z.most_units * d.cache.kv_heads;
     };
-    const auto join = [&](const PagedAttentionShape &z) {
-        // a tile of several units has two at least
-        const uint32_t cut = z.most_units - z.most_tiles, tiles = cut < z.most_tiles ? cut : z.most_tiles, rows = d.max_tokens * d.group;
-        paged_attention_join<DP><<<dim3(tiles * d.cache.kv_heads, rows < 8 ? rows : 8), kWaves * kWave, 0, s>>>(a);
+    // a tile of several units has two at least
+    const auto cut_tiles = [&](const PagedAttentionShape &z) {
+        const uint32_t cut = z.most_units - z.most_tiles;
+        return (cut < z.most_tiles ? cut : z.most_tiles) * d.cache.kv_heads;
     };
     if (d.few.most_tiles != 0) {
         const unsigned units = shape(d.few);
@@ -528,14 +528,14 @@ void launch(const PagedAttentionAmdDescriptor &d, AttentionArgs a, hipStream_t s
         } else {
             paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
         }
-        join(d.few);
+        const uint32_t rows = d.max_tokens * d.group;
+        paged_attention_join<DP><<<dim3(cut_tiles(d.few), rows < 8 ? rows : 8), kWaves * kWave, 0, s>>>(a);
     }
     if (d.many.most_tiles != 0) {
         const unsigned units = shape(d.many);
         a.least_steps = 16;
         a.whole_steps = 2;
-        amdLaunchPagedAttentionTiles(a, FP8, units, s);
-        join(d.many);
+        amdLaunchPagedAttentionTiles(a, FP8, units, cut_tiles(d.many), s);
     }
 }
 

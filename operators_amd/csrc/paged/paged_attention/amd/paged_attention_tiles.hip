@@ -27,6 +27,46 @@ __device__ __forceinline__ float pair_max(float v) {
     return across32(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// What a wavefront's 32 query rows are: rows of the tile from `row0` on, tokens and heads of q and out.
+struct TileRows {
+    uint32_t row0, count, first, head;// count: how many there are of the 32
+};
+
+// 32 rows of q or out between memory, 16 bytes a lane and whole rows by neighbouring lanes, and LDS, a row every RP bytes.
+template<int DP>
+constexpr int kRowPitch = DP * 2 + 16;
+
+template<int DP, typename F>
+__device__ __forceinline__ void each_piece(const AttentionArgs &a, const TileRows &t, uint32_t lane, int64_t token_step, int64_t head_step, F f) {
+    constexpr int PIECES = DP / 8;
+#pragma unroll
+    for (int j = 0; j < 32 * PIECES / kWave; ++j) {
+        const uint32_t index = lane + j * kWave, row = index / PIECES, piece = index % PIECES;
+        const uint32_t r = t.row0 + row, token = fast_quotient(r, a.by_group);
+        f(j, row < t.count && piece * 8 < a.dim, row * kRowPitch<DP> + piece * 16,
+          static_cast<int64_t>(t.first + token) * token_step + static_cast<int64_t>(t.head * a.group + (r - token * a.group)) * head_step + piece * 8);
+    }
+}
+
+// O times `by` to out, through LDS.  o[t][i] of lane (n, h) is column TD m' + t of row n, m' = 8 (i / 4) + 4 h + i % 4.
+template<int DP>
+__device__ __forceinline__ void put_rows(const AttentionArgs &a, const TileRows &rows, uint32_t lane, uint8_t *scratch, const f32x16 (&o)[DP / 32], float by) {
+    constexpr int TD = DP / 32;
+    const uint32_t n32 = lane & 31u, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+        for (int t = 0; t < TD; t += 2) {
+            *reinterpret_cast<uint32_t *>(scratch + n32 * kRowPitch<DP> + ((8 * (i / 4) + 4 * h + i % 4) * TD + t) * 2) =
+                narrow2_rne(a.bf16, o[t][i] * by, o[t + 1][i] * by);
+        }
+    }
+    each_piece<DP>(a, rows, lane, a.out_token, a.out_head, [&](int, bool there, uint32_t in_lds, int64_t at) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(scratch + in_lds);
+        if (there) st16_any(a.out + at, w);
+    });
+}
+
 template<bool FP8, int DP>
 __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_tiles(AttentionArgs a) {
     constexpr int kWaves = paged_tile_waves(DP), kLanes = kWaves * kWave;
@@ -37,8 +77,8 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     constexpr int K_TASKS = BK * NC, V_TASKS = BK / 4 * (DP / 4);
     static_assert(K_TASKS == V_TASKS, "as many pieces of K as of V");
     constexpr int PER = (K_TASKS + kLanes - 1) / kLanes;// of a lane
-    __shared__ __attribute__((aligned(16))) uint8_t k_lds[2][BK * KP];
-    __shared__ __attribute__((aligned(16))) uint8_t v_lds[2][DP * VP];
+    constexpr int TILES = 2 * (BK * KP + DP * VP), ROWS = kWaves * 32 * kRowPitch<DP>;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[TILES > ROWS ? TILES : ROWS];// two tiles; before and after, the query rows
     __shared__ uint64_t slots[kWaves];
     __shared__ Unit shared_unit;
     Unit u;
@@ -54,25 +94,146 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     // this wavefront's rows, and what its first and its last see
     const uint32_t mine0 = row0 + wave * 32, mine1 = mine0 + 32 < row_end ? mine0 + 32 : row_end;
     const bool any = mine0 < row_end;
+    const TileRows my_rows{mine0, any ? mine1 - mine0 : 0, u.first, head};
     const uint32_t all_see = any ? sees(fast_quotient(mine0, a.by_group)) : 0, some_see = any ? sees(fast_quotient(mine1 - 1, a.by_group)) : 0;
     const uint32_t tile_sees = sees(fast_quotient(row_end - 1, a.by_group));
+    const uint32_t limit = mine0 + n32 < row_end ? sees(fast_quotient(mine0 + n32, a.by_group)) : 0;
+    uint8_t *const scratch = lds + wave * 32 * kRowPitch<DP>;
+    const auto k_lds = [&](uint32_t tile) { return lds + (tile & 1u) * (BK * KP); };
+    const auto v_lds = [&](uint32_t tile) { return lds + 2 * BK * KP + (tile & 1u) * (DP * VP); };
 
-    const uint32_t r = mine0 + n32, token = fast_quotient(r, a.by_group);
-    const bool mine = r < row_end;
-    const uint32_t limit = mine ? sees(token) : 0;
-    const int64_t q_head = static_cast<int64_t>(head * a.group + (r - token * a.group));
-    // the query row as the second operand: piece 2 s + h of K's order in LDS at step s
+    const uint32_t end = (tile_sees + kStepKeys - 1) / kStepKeys;
+    const uint32_t s0 = u.chunk * u.steps, s1 = s0 + u.steps < end ? s0 + u.steps : end;
+    const uint32_t first_key = s0 * kStepKeys, tiles = s1 > s0 ? (s1 - s0 + NB - 1) / NB : 0;
+    const uint32_t my_tiles = some_see <= first_key ? 0 : (some_see - first_key + BK - 1) / BK < tiles ? (some_see - first_key + BK - 1) / BK : tiles;
+
+    // a lane's pieces of a tile: 16 bytes of one key of K, 4 bytes of 4 keys of V
+    const auto k_key = [&](int i) { return (tid + i * kLanes) / NC; };
+    const auto k_piece = [&](int i) { return (tid + i * kLanes) % NC; };
+    const auto v_keys = [&](int i) { return (tid + i * kLanes) / (DP / 4) * 4; };
+    const auto v_col = [&](int i) { return (tid + i * kLanes) % (DP / 4) * 4; };
+    const auto works = [&](int i) { return K_TASKS % kLanes == 0 || tid + i * kLanes < K_TASKS; };
+    // (the 16 keys it is of: the same for the whole wavefront, for 16 keys are the pieces of whole wavefronts, or a
+    // wavefront's pieces lie within 16 keys)
+    const auto group_of = [](uint32_t key) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(key / 16))); };
+    uint32_t k_off[PER], v_off[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        k_off[i] = (k_key(i) & 15u) * a.k_at.token + (k_piece(i) * 16 < a.dim ? k_piece(i) * 16 : 0);// (q is 0 behind dim)
+        v_off[i] = (v_keys(i) & 15u) * a.v_at.token + (v_col(i) < a.dim ? v_col(i) : 0);             // (not stored behind dim)
+    }
+    const uint8_t *k_base = a.k + static_cast<uint64_t>(head) * a.k_at.head, *v_base = a.v + static_cast<uint64_t>(head) * a.v_at.head;
+    const float *ks_base = a.k_scale + static_cast<int64_t>(head) * a.k_at.s_head, *vs_base = a.v_scale + static_cast<int64_t>(head) * a.v_at.s_head;
+    const int *table = a.rows.table + u.row * a.rows.stride;
+
+    // What tiles are loaded and computed with is read for 64 groups of 16 keys at once, one for each lane: the pages, ahead
+    // for K and for V, and for the computation the scales.
+    constexpr uint32_t kAhead = 64 / NG;// tiles of such a set
+    const auto page_of = [&](uint32_t tile) {
+        const uint32_t key = first_key + tile * BK + lane * 16;
+        if (key >= u.length) return -1;
+        const int page = table[fast_quotient(key, a.rows.by_page)];
+        return static_cast<uint32_t>(page) < a.pages ? page : -1;
+    };
+    const auto place_of = [&](uint32_t key) { return key - fast_quotient(key, a.rows.by_page) * a.rows.page; };
+    const auto lane_of = [](float v, uint32_t l2) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l2)); };
+    int k_pages = page_of(0), v_pages = k_pages;
+    u32x4 k_raw[PER];
+    uint32_t v_raw[PER][4];
+    const auto load_k = [&](uint32_t tile) {
+        if (tile % kAhead == 0 && tile != 0) k_pages = page_of(tile);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (!works(i)) continue;
+            const uint32_t g = group_of(k_key(i));
+            const int pg = __builtin_amdgcn_readlane(k_pages, tile % kAhead * NG + g);
+            k_raw[i] = ld16(k_base + static_cast<int64_t>(pg < 0 ? 0 : pg) * a.k_at.page +
+                            static_cast<uint64_t>(place_of(first_key + tile * BK + g * 16)) * a.k_at.token + k_off[i]);
+        }
+    };
+    const auto load_v = [&](uint32_t tile) {
+        if (tile % kAhead == 0 && tile != 0) v_pages = page_of(tile);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (!works(i)) continue;
+            const uint32_t g = group_of(v_keys(i));
+            const int pg = __builtin_amdgcn_readlane(v_pages, tile % kAhead * NG + g);
+            const uint8_t *p = v_base + static_cast<int64_t>(pg < 0 ? 0 : pg) * a.v_at.page +
+                               static_cast<uint64_t>(place_of(first_key + tile * BK + g * 16)) * a.v_at.token;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v_raw[i][j] = *reinterpret_cast<const uint32_t *>(p + static_cast<uint64_t>(j) * a.v_at.token + v_off[i]);
+        }
+    };
+    const auto store_k = [&](uint32_t tile) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (!works(i)) continue;
+            uint8_t *k = k_lds(tile) + k_key(i) * KP + k_piece(i) * 16;
+            f16x8 half[2];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t c = prepare_codes<FP8>(k_raw[i][w]);
+                const f16x2 x = pair_of<FP8, false>(c), y = pair_of<FP8, true>(c);
+                f16x8 &to = half[w / 2];
+                to[w % 2 * 4] = x.x;
+                to[w % 2 * 4 + 1] = x.y;
+                to[w % 2 * 4 + 2] = y.x;
+                to[w % 2 * 4 + 3] = y.y;
+            }
+            *reinterpret_cast<f16x8 *>(k) = half[0];
+            *reinterpret_cast<f16x8 *>(k + NC * 16) = half[1];
+        }
+    };
+    const auto store_v = [&](uint32_t tile) {// before the V of another tile is loaded
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (!works(i)) continue;
+            uint32_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = v_raw[i][j];
+            // what lies behind the row's end, or in no page, may be anything: no number times 0 is 0
+            const bool none = __builtin_amdgcn_readlane(v_pages, tile % kAhead * NG + group_of(v_keys(i))) < 0;
+            if (none || first_key + tile * BK + BK > u.length) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = none || first_key + tile * BK + v_keys(i) + j >= u.length ? 0 : x[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = prepare_codes<FP8>(x[j]);
+            uint32_t pair[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                pair[j][0] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05010400u);
+                pair[j][1] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07030602u);
+            }
+            // 16 keys in order of the accumulator's halves: 0-3, 8-11, 4-7, 12-15
+            const uint32_t quad = v_keys(i) / 4 & 3u, place = (v_keys(i) & ~15u) + (quad & 1u) * 8 + (quad >> 1) * 4;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const auto two = [&](int j) { return __builtin_bit_cast(uint32_t, c % 2 ? pair_of<FP8, true>(pair[j][c / 2]) : pair_of<FP8, false>(pair[j][c / 2])); };
+                // column d is row d / TD of the accumulator's tile d % TD
+                const uint32_t d = v_col(i) + c, row = d % TD * 32 + d / TD;
+                *reinterpret_cast<u32x2 *>(v_lds(tile) + row * VP + place * 2) = u32x2{two(0), two(1)};
+            }
+        }
+    };
+    load_k(0);
+    load_v(0);
+
+    // the query rows as the second operand: piece 2 s + h of K's order in LDS at step s
     f16x8 q[KS];
     float factor;
     {
         u32x4 w[KS];
-        const uint16_t *p = a.q + static_cast<int64_t>(u.first + token) * a.q_token + q_head * a.q_head;
+        each_piece<DP>(a, my_rows, lane, a.q_token, a.q_head, [&](int j, bool there, uint32_t, int64_t at) {
+            w[j] = u32x4{0, 0, 0, 0};
+            if (there) w[j] = ld16_any(a.q + at);
+        });
+        each_piece<DP>(a, my_rows, lane, 0, 0, [&](int j, bool, uint32_t in_lds, int64_t) { *reinterpret_cast<u32x4 *>(scratch + in_lds) = w[j]; });
         float top = 0.0f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const uint32_t piece = 2 * s + h, d = piece % NC * 16 + piece / NC * 8;
-            w[s] = u32x4{0, 0, 0, 0};
-            if (mine && d < a.dim) w[s] = ld16_any(p + d);
+            const uint32_t piece = 2 * s + h, d8 = piece % NC * 2 + piece / NC;
+            w[s] = *reinterpret_cast<const u32x4 *>(scratch + n32 * kRowPitch<DP> + d8 * 16);
             float x[8];
             if (a.bf16) widen8<BF16Rne>(w[s], x);
             else widen8<F16Ref>(w[s], x);
@@ -100,150 +261,44 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     }
     // the running maximum less 10, its sum, and log2 of the largest V scale so far, which O stands relative to
     float m = kNone, l = 0.0f, v_top = kNone;
-
-    // a lane's pieces of a tile: 16 bytes of one key of K, 4 bytes of 4 keys of V
-    const auto k_key = [&](int i) { return (tid + i * kLanes) / NC; };
-    const auto k_piece = [&](int i) { return (tid + i * kLanes) % NC; };
-    const auto v_keys = [&](int i) { return (tid + i * kLanes) / (DP / 4) * 4; };
-    const auto v_col = [&](int i) { return (tid + i * kLanes) % (DP / 4) * 4; };
-    const auto works = [&](int i) { return K_TASKS % kLanes == 0 || tid + i * kLanes < K_TASKS; };
-    // (the 16 keys it is of: the same for the whole wavefront, for 16 keys are the pieces of whole wavefronts, or a
-    // wavefront's pieces lie within 16 keys)
-    const auto group_of = [](uint32_t key) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(key / 16))); };
-    uint32_t k_off[PER], v_off[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        k_off[i] = (k_key(i) & 15u) * a.k_at.token + (k_piece(i) * 16 < a.dim ? k_piece(i) * 16 : 0);// (q is 0 behind dim)
-        v_off[i] = (v_keys(i) & 15u) * a.v_at.token + (v_col(i) < a.dim ? v_col(i) : 0);             // (not stored behind dim)
-    }
-    const uint8_t *k_base = a.k + static_cast<uint64_t>(head) * a.k_at.head, *v_base = a.v + static_cast<uint64_t>(head) * a.v_at.head;
-    const float *ks_base = a.k_scale + static_cast<int64_t>(head) * a.k_at.s_head, *vs_base = a.v_scale + static_cast<int64_t>(head) * a.v_at.s_head;
-    const int *table = a.rows.table + u.row * a.rows.stride;
-
-    const uint32_t end = (tile_sees + kStepKeys - 1) / kStepKeys;
-    const uint32_t s0 = u.chunk * u.steps, s1 = s0 + u.steps < end ? s0 + u.steps : end;
-    const uint32_t first_key = s0 * kStepKeys, tiles = s1 > s0 ? (s1 - s0 + NB - 1) / NB : 0;
-    const uint32_t my_tiles = some_see <= first_key ? 0 : (some_see - first_key + BK - 1) / BK < tiles ? (some_see - first_key + BK - 1) / BK : tiles;
-
-    // What a tile is loaded and computed with is read for 64 groups of 16 keys at once, one for each lane: their pages
-    // for K and for V, which are loaded three and two tiles ahead, and pages and scales for the computation.
-    constexpr uint32_t kAhead = 64 / NG;// tiles of such a set
-    const auto page_of = [&](uint32_t tile) {
-        const uint32_t key = first_key + tile * BK + lane * 16;
-        if (key >= u.length) return -1;
-        const int page = table[fast_quotient(key, a.rows.by_page)];
-        return static_cast<uint32_t>(page) < a.pages ? page : -1;
-    };
-    const auto place_of = [&](uint32_t key) { return key - fast_quotient(key, a.rows.by_page) * a.rows.page; };
-    int k_pages = -1, v_pages = -1, page = -1;
-    float k_scale = 0.0f, v_log = kNone;
+    float k_scale, v_rel, v_back;// of the lane's group: of V log2 relative to v_top, and the way back
+    uint64_t no_page = 0;        // a bit for each group
     const auto scales = [&](uint32_t tile) {
-        page = page_of(tile);
+        const int page = page_of(tile);
+        float v_log = -200.0f;
         k_scale = 0.0f;
-        v_log = -200.0f;
         if (page >= 0) {
             const uint32_t block = fast_quotient(place_of(first_key + tile * BK + lane * 16), a.by_block);
             k_scale = ks_base[page * a.k_at.s_page + block];
             v_log = __builtin_amdgcn_logf(fmaxf(vs_base[page * a.v_at.s_page + block], 0x1p-126f));
         }
-    };
-    const auto lane_of = [](float v, uint32_t l2) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l2)); };
-
-    u32x4 k_raw[PER];
-    uint32_t v_raw[PER][4];
-    int v_live[PER];// how many of the 4 keys there are
-    const auto load_k = [&](uint32_t tile) {
-        if (tile % kAhead == 0) k_pages = page_of(tile);
+        no_page = __builtin_amdgcn_ballot_w64(page < 0);
+        const float v_now = wave_max(v_log);
+        if (v_now > v_top) {
+            const float by = __builtin_amdgcn_exp2f(v_top - v_now);
+            v_top = v_now;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if (!works(i)) continue;
-            const uint32_t g = group_of(k_key(i));
-            const int pg = __builtin_amdgcn_readlane(k_pages, tile % kAhead * NG + g);
-            k_raw[i] = ld16(k_base + static_cast<int64_t>(pg < 0 ? 0 : pg) * a.k_at.page +
-                            static_cast<uint64_t>(place_of(first_key + tile * BK + g * 16)) * a.k_at.token + k_off[i]);
+            for (int t = 0; t < TD; ++t) o[t] *= by;
         }
-    };
-    const auto load_v = [&](uint32_t tile) {
-        if (tile % kAhead == 0) v_pages = page_of(tile);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if (!works(i)) continue;
-            const uint32_t g = group_of(v_keys(i));
-            const int pg = __builtin_amdgcn_readlane(v_pages, tile % kAhead * NG + g);
-            const uint8_t *p = v_base + static_cast<int64_t>(pg < 0 ? 0 : pg) * a.v_at.page +
-                               static_cast<uint64_t>(place_of(first_key + tile * BK + g * 16)) * a.v_at.token;
-            v_live[i] = pg < 0 ? 0 : static_cast<int>(u.length) - static_cast<int>(first_key + tile * BK + v_keys(i));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v_raw[i][j] = *reinterpret_cast<const uint32_t *>(p + static_cast<uint64_t>(j) * a.v_at.token + v_off[i]);
-        }
-    };
-    const auto store_k = [&](uint32_t tile) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if (!works(i)) continue;
-            uint8_t *k = k_lds[tile & 1u] + k_key(i) * KP + k_piece(i) * 16;
-            f16x8 half[2];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const uint32_t c = prepare_codes<FP8>(k_raw[i][w]);
-                const f16x2 x = pair_of<FP8, false>(c), y = pair_of<FP8, true>(c);
-                f16x8 &to = half[w / 2];
-                to[w % 2 * 4] = x.x;
-                to[w % 2 * 4 + 1] = x.y;
-                to[w % 2 * 4 + 2] = y.x;
-                to[w % 2 * 4 + 3] = y.y;
-            }
-            *reinterpret_cast<f16x8 *>(k) = half[0];
-            *reinterpret_cast<f16x8 *>(k + NC * 16) = half[1];
-        }
-    };
-    const auto store_v = [&](uint32_t tile) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if (!works(i)) continue;
-            uint32_t x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = v_raw[i][j];
-            // what lies behind the row's end, or in no page, may be anything: no number times 0 is 0
-            if (__builtin_amdgcn_ballot_w64(v_live[i] < 4) != 0) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = j >= v_live[i] ? 0 : x[j];
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = prepare_codes<FP8>(x[j]);
-            uint32_t pair[2][2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                pair[j][0] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05010400u);
-                pair[j][1] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07030602u);
-            }
-            // 16 keys in order of the accumulator's halves: 0-3, 8-11, 4-7, 12-15
-            const uint32_t quad = v_keys(i) / 4 & 3u, place = (v_keys(i) & ~15u) + (quad & 1u) * 8 + (quad >> 1) * 4;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const auto two = [&](int j) { return __builtin_bit_cast(uint32_t, c % 2 ? pair_of<FP8, true>(pair[j][c / 2]) : pair_of<FP8, false>(pair[j][c / 2])); };
-                // column d is row d / TD of the accumulator's tile d % TD
-                const uint32_t d = v_col(i) + c, row = d % TD * 32 + d / TD;
-                *reinterpret_cast<u32x2 *>(v_lds[tile & 1u] + row * VP + place * 2) = u32x2{two(0), two(1)};
-            }
-        }
+        v_rel = fmaxf(v_log - v_top, kLeastRatio);
+        v_back = __builtin_amdgcn_exp2f(-v_rel);
     };
 
     // The scores of a tile as the matrix units leave them, and what they are multiplied by.
     f32x16 s[NB];
     float f[NG], high = kNone;
-    const auto products = [&](uint32_t tile, f32x16(&x)[NB]) {
+    const auto products = [&](uint32_t tile) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[b][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < KS; ++e) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const f16x8 k = *reinterpret_cast<const f16x8 *>(k_lds[tile & 1u] + (b * 32 + n32) * KP + (2 * e + h) * 16);
-                x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], x[b], 0, 0, 0);
+                const f16x8 k = *reinterpret_cast<const f16x8 *>(k_lds(tile) + (b * 32 + n32) * KP + (2 * e + h) * 16);
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], s[b], 0, 0, 0);
             }
         }
     };
@@ -261,33 +316,21 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             high = fmaxf(high, top * f[g]);
         }
     };
-    // What a tile's scores need before their exponentials: its scales, the mask, the maximum, the V scale.
+    // What a tile's scores need before their exponentials: the mask and the maximum.
     const auto ready = [&](uint32_t tile) {
-        const uint32_t key0 = first_key + tile * BK, at = tile % kAhead * NG;
-        float v_now = kNone;
-        int least = 0;// below 0: a group without a page
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            least |= __builtin_amdgcn_readlane(page, at + g);
-            v_now = fmaxf(v_now, lane_of(v_log, at + g));
-        }
-        if (least < 0 || key0 + BK > all_see) {
+        const uint32_t key0 = first_key + tile * BK;
+        const uint32_t none = static_cast<uint32_t>(no_page >> (tile % kAhead * NG)) & ((1u << NG) - 1);
+        if (none != 0 || key0 + BK > all_see) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const uint32_t key = key0 + b * 32 + 8 * (i / 4) + 4 * h + i % 4;
-                    const bool gone = (key >= limit) | (__builtin_amdgcn_readlane(page, at + 2 * b + i / 8) < 0);
+                    const bool gone = key >= limit || (none >> (2 * b + i / 8) & 1u) != 0;
                     s[b][i] = gone ? -__builtin_inff() : s[b][i];
                 }
             }
             largest(tile);
-        }
-        if (v_now > v_top + 1.0f) {
-            const float by = __builtin_amdgcn_exp2f(v_top - v_now);
-            v_top = v_now;
-#pragma unroll
-            for (int t = 0; t < TD; ++t) o[t] *= by;
         }
         if (__builtin_amdgcn_ballot_w64(high > m + (kLift + kSlack)) != 0) {
             const float next = fmaxf(m, pair_max(high) - kLift), by = __builtin_amdgcn_exp2f(m - next);
@@ -298,43 +341,52 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         }
     };
 
+    // Of eight wavefronts, two on each SIMD, the second four are a phase behind the first: while these use the matrix
+    // units, those use the vector units for exponentials and for the codes on their way into LDS.  A barrier a phase.
+    // What the first four write is needed in their next phase, what the others write in the phase after that.
+    constexpr bool kTurns = kWaves == 8;
+    const uint32_t lead = kTurns && wave < 4 ? 1 : 2;// K of tile + lead and V of the one before are written beside tile's exponentials
     if (tiles != 0) {
-        load_k(0);
-        store_k(0);
-        load_v(0);
-        if (tiles > 1) {
-            load_k(1);
-            store_k(1);
-        }
-        store_v(0);
-        if (tiles > 2) load_k(2);
-        if (tiles > 1) load_v(1);
         scales(0);
+        __syncthreads();// the query rows are read
+        store_k(0);
+        if (lead == 2) {
+            store_v(0);
+            if (tiles > 1) {
+                load_k(1);
+                store_k(1);
+                load_v(1);
+            }
+            if (tiles > 2) load_k(2);
+        } else if (tiles > 1) {
+            load_k(1);
+        }
         __syncthreads();
         if (my_tiles != 0) {
-            products(0, s);
+            products(0);
             largest(0);
             ready(0);
         }
         __syncthreads();
+        if (kTurns && wave >= 4) __syncthreads();
         for (uint32_t tile = 0; tile < tiles; ++tile) {
-            if (tile + 2 < tiles) store_k(tile + 2);
-            if (tile + 1 < tiles) store_v(tile + 1);
-            if (tile + 3 < tiles) load_k(tile + 3);
-            if (tile + 2 < tiles) load_v(tile + 2);
+            if (tile + lead < tiles) store_k(tile + lead);
+            if (tile + lead - 1 < tiles) store_v(tile + lead - 1);
+            if (tile + lead + 1 < tiles) load_k(tile + lead + 1);
+            if (tile + lead < tiles) load_v(tile + lead);
+            f16x8 p[NG];
             if (tile < my_tiles) {
                 const uint32_t at = tile % kAhead * NG;
-                f16x8 p[NG];
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const float v = fmaxf(lane_of(v_log, at + g) - v_top, kLeastRatio), less = v - m;
+                    const float less = lane_of(v_rel, at + g) - m;
                     float y[8], sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + i], f[g], less));
                         sum += y[i];
                     }
-                    l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-v), l);
+                    l = __builtin_fmaf(sum, lane_of(v_back, at + g), l);
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) {
                         const f16x2 w = __builtin_convertvector((f32x2{y[i], y[i + 1]}), f16x2);
@@ -342,73 +394,112 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
                         p[g][i + 1] = w.y;
                     }
                 }
-                if ((tile + 1) % kAhead == 0) scales(tile + 1);
-                // the next tile's products, beside this one's exponentials (behind the last they are not used)
-                f32x16 next[NB];
-                products(tile + 1, next);
+            }
+            if (kTurns) __syncthreads();
+            if (tile < my_tiles) {
+                // the next tile's products (behind the last they are not used), and this one's sums
+                if (kTurns) __builtin_amdgcn_s_setprio(1);
+                products(tile + 1);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
 #pragma unroll
                     for (int t = 0; t < TD; ++t) {
-                        const f16x8 x = *reinterpret_cast<const f16x8 *>(v_lds[tile & 1u] + (t * 32 + n32) * VP + g * 32 + h * 16);
+                        const f16x8 x = *reinterpret_cast<const f16x8 *>(v_lds(tile) + (t * 32 + n32) * VP + g * 32 + h * 16);
                         o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p[g], o[t], 0, 0, 0);
                     }
                 }
+                // eight operands are on their way from LDS while the matrix units are at work
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) s[b] = next[b];
+                for (int i = 0; i < (KS * NB + NG * TD) - 8; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
+                if (kTurns) __builtin_amdgcn_s_setprio(0);
+                if ((tile + 1) % kAhead == 0) scales(tile + 1);
                 largest(tile + 1);
                 if (tile + 1 < my_tiles) ready(tile + 1);
             }
             __syncthreads();
         }
+        if (kTurns && wave < 4) __syncthreads();
     }
-    const float v_unit = __builtin_amdgcn_exp2f(fmaxf(v_top, -140.0f));
 
-    if (!mine) return;
-    l = across32(l, [](float x, float y) { return x + y; });// (the other half of a row is in the same wavefront, and stays or goes with it)
-    // o[t][i] is column TD m' + t of the row, m' = 8 (i / 4) + 4 h + i % 4
-    if (u.chunks > 1) {
-        const uint64_t at = (static_cast<uint64_t>(u.slot + u.chunk) * a.kv_heads + head) * a.tile_rows + wave * 32 + n32;
+    if (!any) return;
+    l = across32(l, [](float x, float y) { return x + y; });
+    const float v_unit = __builtin_amdgcn_exp2f(fmaxf(v_top, -140.0f));
+    if (u.chunks > 1) {// as the lanes hold it, 16 bytes of each side by side
+        const uint64_t at = (static_cast<uint64_t>(u.slot + u.chunk) * a.kv_heads + head) * kWaves + wave;
         if (h == 0) {
-            a.part_stat[2 * at] = m;
-            a.part_stat[2 * at + 1] = l;
+            a.part_stat[2 * (at * 32 + n32)] = m;
+            a.part_stat[2 * (at * 32 + n32) + 1] = l;
         }
-        // (where l is 0 it is not read)
+        float *p = a.part_out + at * (32 * DP) + lane * 4;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float *p = a.part_out + at * DP + (8 * (i / 4) + 4 * h + i % 4) * TD;
-#pragma unroll
-            for (int t = 0; t < TD; t += 2) *reinterpret_cast<f32x2 *>(p + t) = f32x2{o[t][i] * v_unit, o[t + 1][i] * v_unit};
+        for (int k = 0; k < 16 * TD; k += 4) {
+            const auto of = [&](int j) { return o[(k + j) % TD][(k + j) / TD] * v_unit; };
+            *reinterpret_cast<f32x4 *>(p + k * kWave) = f32x4{of(0), of(1), of(2), of(3)};
         }
     } else {
-        const float by = l > 0.0f ? v_unit / l : 0.0f;
-        uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + q_head * a.out_head;
-        typedef uint32_t __attribute__((aligned(2))) u32_any;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint32_t d = (8 * (i / 4) + 4 * h + i % 4) * TD;
-#pragma unroll
-            for (int t = 0; t < TD; t += 2) {
-                if (d + t < a.dim) *reinterpret_cast<u32_any *>(p + d + t) = narrow2_rne(a.bf16, o[t][i] * by, o[t + 1][i] * by);
-            }
-        }
+        put_rows<DP>(a, my_rows, lane, scratch, o, l > 0.0f ? v_unit / l : 0.0f);
     }
+}
+
+// The units of a tile together, a wavefront for 32 query rows, in the lanes that held them.
+template<int DP>
+__global__ __launch_bounds__(kWave) void paged_attention_tiles_join(AttentionArgs a) {
+    constexpr int TD = DP / 32;
+    __shared__ __attribute__((aligned(16))) uint8_t scratch[32 * kRowPitch<DP>];
+    __shared__ uint64_t slots[1];
+    __shared__ Unit shared_unit;
+    Unit u;
+    const uint32_t waves = a.tile_rows / 32, wave = blockIdx.x % waves, head = blockIdx.x / waves % a.kv_heads;
+    if (!find_unit<1, true>(a, blockIdx.x / waves / a.kv_heads, slots, &shared_unit, &u)) return;
+    const uint32_t lane = threadIdx.x, n32 = lane & 31u;
+    const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens, rows = tokens * a.group, mine0 = u.tile * a.tile_rows + wave * 32;
+    if (mine0 >= rows) return;
+    const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * waves + wave; };
+    float high = kNone;
+    for (uint32_t c = 0; c < u.chunks; ++c) high = fmaxf(high, a.part_stat[2 * (at(c) * 32 + n32)]);
+    f32x16 o[TD];
+#pragma unroll
+    for (int t = 0; t < TD; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    }
+    float total = 0.0f;
+#pragma unroll 1
+    for (uint32_t c = 0; c < u.chunks; ++c) {
+        f32x4 x[4 * TD];
+        const float *p = a.part_out + at(c) * (32 * DP) + lane * 4;
+#pragma unroll
+        for (int k = 0; k < 4 * TD; ++k) x[k] = ld16f(p + k * 4 * kWave);
+        const float l = a.part_stat[2 * (at(c) * 32 + n32) + 1], by = __builtin_amdgcn_exp2f(a.part_stat[2 * (at(c) * 32 + n32)] - high);
+        total += l * by;
+#pragma unroll
+        for (int k = 0; k < 16 * TD; ++k) o[k % TD][k / TD] += x[k / 4][k % 4] * by;
+    }
+    put_rows<DP>(a, TileRows{mine0, rows - mine0 < 32 ? rows - mine0 : 32, u.first, head}, lane, scratch, o, total > 0.0f ? 1.0f / total : 0.0f);
 }
 
 template<bool FP8, int DP>
-void launch(const AttentionArgs &a, unsigned units, hipStream_t s) {
+void launch(const AttentionArgs &a, unsigned units, unsigned cut_tiles, hipStream_t s) {
     paged_attention_tiles<FP8, DP><<<units, paged_tile_waves(DP) * kWave, 0, s>>>(a);
+    paged_attention_tiles_join<DP><<<cut_tiles * paged_tile_waves(DP), kWave, 0, s>>>(a);
 }
 template<bool FP8>
-void launch(const AttentionArgs &a, unsigned units, hipStream_t s) {
+void launch(const AttentionArgs &a, unsigned units, unsigned cut_tiles, hipStream_t s) {
     switch (paged_dim(a.dim)) {
-        case 64: return launch<FP8, 64>(a, units, s);
-        case 128: return launch<FP8, 128>(a, units, s);
-        case 192: return launch<FP8, 192>(a, units, s);
-        default: return launch<FP8, 256>(a, units, s);
+        case 64: return launch<FP8, 64>(a, units, cut_tiles, s);
+        case 128: return launch<FP8, 128>(a, units, cut_tiles, s);
+        case 192: return launch<FP8, 192>(a, units, cut_tiles, s);
+        default: return launch<FP8, 256>(a, units, cut_tiles, s);
     }
 }
 
 }// namespace
 
-void amdLaunchPagedAttentionTiles(const AttentionArgs &a, bool fp8, unsigned units, hipStream_t s) { fp8 ? launch<true>(a, units, s) : launch<false>(a, units, s); }
+void amdLaunchPagedAttentionTiles(const AttentionArgs &a, bool fp8, unsigned units, unsigned cut_tiles, hipStream_t s) {
+    fp8 ? launch<true>(a, units, cut_tiles, s) : launch<false>(a, units, cut_tiles, s);
+}

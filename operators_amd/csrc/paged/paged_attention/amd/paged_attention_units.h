@@ -171,7 +171,7 @@ __device__ __forceinline__ uint32_t narrow2_rne(bool bf16, float a, float b) {
 
 }// namespace amd
 
-// paged_attention_tiles.hip: many query rows
-void amdLaunchPagedAttentionTiles(const amd::AttentionArgs &a, bool fp8, unsigned units, hipStream_t s);
+// paged_attention_tiles.hip: many query rows.  `units` workgroups, and for what joins them the most tiles that are cut.
+void amdLaunchPagedAttentionTiles(const amd::AttentionArgs &a, bool fp8, unsigned units, unsigned cut_tiles, hipStream_t s);
 
 #endif
