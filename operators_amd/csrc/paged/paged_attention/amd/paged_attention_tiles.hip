@@ -272,6 +272,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             k_scale = ks_base[page * a.k_at.s_page + block];
             v_log = __builtin_amdgcn_logf(fmaxf(vs_base[page * a.v_at.s_page + block], 0x1p-126f));
         }
+        asm volatile("" : "+v"(k_scale));// (waited for here, not where this way and the one past it meet)
         no_page = __builtin_amdgcn_ballot_w64(page < 0);
         const float v_now = wave_max(v_log);
         if (v_now > v_top) {
@@ -350,16 +351,12 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         scales(0);
         __syncthreads();// the query rows are read
         store_k(0);
+        load_k(1);
         if (lead == 2) {
             store_v(0);
-            if (tiles > 1) {
-                load_k(1);
-                store_k(1);
-                load_v(1);
-            }
-            if (tiles > 2) load_k(2);
-        } else if (tiles > 1) {
-            load_k(1);
+            load_v(1);
+            store_k(1);
+            load_k(2);
         }
         __syncthreads();
         if (my_tiles != 0) {
@@ -370,10 +367,12 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         __syncthreads();
         if (kTurns && wave >= 4) __syncthreads();
         for (uint32_t tile = 0; tile < tiles; ++tile) {
-            if (tile + lead < tiles) store_k(tile + lead);
-            if (tile + lead - 1 < tiles) store_v(tile + lead - 1);
-            if (tile + lead + 1 < tiles) load_k(tile + lead + 1);
-            if (tile + lead < tiles) load_v(tile + lead);
+            // (also behind the last tile, where nobody reads what is written: a condition here would make the compiler wait for
+            // all loads where the ways meet)
+            store_k(tile + lead);
+            store_v(tile + lead - 1);
+            load_k(tile + lead + 1);
+            load_v(tile + lead);
             f16x8 p[NG];
             if (tile < my_tiles) {
                 const uint32_t at = tile % kAhead * NG;
