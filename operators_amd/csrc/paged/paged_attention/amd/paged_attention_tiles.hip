@@ -137,31 +137,45 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     };
     const auto place_of = [&](uint32_t key) { return key - fast_quotient(key, a.rows.by_page) * a.rows.page; };
     const auto lane_of = [](float v, uint32_t l2) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l2)); };
-    int k_pages = page_of(0), v_pages = k_pages;
+    const auto lane_of64 = [](uint64_t v, uint32_t l2) {
+        return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l2)) |
+               static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), l2))) << 32;
+    };
+    // where a group's first key is; no page: page 0, for any place will do
+    const auto bytes_of = [&](uint32_t tile, int page, const PagedStrides &at) {
+        return static_cast<uint64_t>(static_cast<int64_t>(page < 0 ? 0 : page) * at.page) +
+               static_cast<uint64_t>(place_of(first_key + tile * BK + lane * 16)) * at.token;
+    };
+    uint64_t k_group, v_group, v_none;// v_none: a bit for each group without a page
+    {
+        const int page = page_of(0);
+        k_group = bytes_of(0, page, a.k_at);
+        v_group = bytes_of(0, page, a.v_at);
+        v_none = __builtin_amdgcn_ballot_w64(page < 0);
+    }
     u32x4 k_raw[PER];
     uint32_t v_raw[PER][4];
     const auto load_k = [&](uint32_t tile) {
-        if (tile % kAhead == 0 && tile != 0) k_pages = page_of(tile);
+        if (tile % kAhead == 0 && tile != 0) k_group = bytes_of(tile, page_of(tile), a.k_at);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (!works(i)) continue;
-            const uint32_t g = group_of(k_key(i));
-            const int pg = __builtin_amdgcn_readlane(k_pages, tile % kAhead * NG + g);
-            k_raw[i] = ld16(k_base + static_cast<int64_t>(pg < 0 ? 0 : pg) * a.k_at.page +
-                            static_cast<uint64_t>(place_of(first_key + tile * BK + g * 16)) * a.k_at.token + k_off[i]);
+            const uint8_t *p = k_base + lane_of64(k_group, tile % kAhead * NG + group_of(k_key(i)));
+            k_raw[i] = ld16(p + k_off[i]);
         }
     };
     const auto load_v = [&](uint32_t tile) {
-        if (tile % kAhead == 0 && tile != 0) v_pages = page_of(tile);
+        if (tile % kAhead == 0 && tile != 0) {
+            const int page = page_of(tile);
+            v_group = bytes_of(tile, page, a.v_at);
+            v_none = __builtin_amdgcn_ballot_w64(page < 0);
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (!works(i)) continue;
-            const uint32_t g = group_of(v_keys(i));
-            const int pg = __builtin_amdgcn_readlane(v_pages, tile % kAhead * NG + g);
-            const uint8_t *p = v_base + static_cast<int64_t>(pg < 0 ? 0 : pg) * a.v_at.page +
-                               static_cast<uint64_t>(place_of(first_key + tile * BK + g * 16)) * a.v_at.token;
+            const uint8_t *p = v_base + lane_of64(v_group, tile % kAhead * NG + group_of(v_keys(i)));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v_raw[i][j] = *reinterpret_cast<const uint32_t *>(p + static_cast<uint64_t>(j) * a.v_at.token + v_off[i]);
+            for (int j = 0; j < 4; ++j, p += a.v_at.token) v_raw[i][j] = *reinterpret_cast<const uint32_t *>(p + v_off[i]);
         }
     };
     const auto store_k = [&](uint32_t tile) {
@@ -192,7 +206,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = v_raw[i][j];
             // what lies behind the row's end, or in no page, may be anything: no number times 0 is 0
-            const bool none = __builtin_amdgcn_readlane(v_pages, tile % kAhead * NG + group_of(v_keys(i))) < 0;
+            const bool none = (v_none >> (tile % kAhead * NG + group_of(v_keys(i))) & 1u) != 0;
             if (none || first_key + tile * BK + BK > u.length) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = none || first_key + tile * BK + v_keys(i) + j >= u.length ? 0 : x[j];
