@@ -54,11 +54,11 @@ __device__ __forceinline__ void put_rows(const AttentionArgs &a, const TileRows 
     constexpr int TD = DP / 32;
     const uint32_t n32 = lane & 31u, h = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 16; i += 4) {
 #pragma unroll
-        for (int t = 0; t < TD; t += 2) {
-            *reinterpret_cast<uint32_t *>(scratch + n32 * kRowPitch<DP> + ((8 * (i / 4) + 4 * h + i % 4) * TD + t) * 2) =
-                narrow2_rne(a.bf16, o[t][i] * by, o[t + 1][i] * by);
+        for (int c = 0; c < 4 * TD; c += 2) {// columns side by side
+            *reinterpret_cast<uint32_t *>(scratch + n32 * kRowPitch<DP> + ((2 * i + 4 * h) * TD + c) * 2) =
+                narrow2_rne(a.bf16, o[c % TD][i + c / TD] * by, o[(c + 1) % TD][i + (c + 1) / TD] * by);
         }
     }
     each_piece<DP>(a, rows, lane, a.out_token, a.out_head, [&](int, bool there, uint32_t in_lds, int64_t at) {
@@ -74,7 +74,8 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     constexpr int KS = DP / 16, NC = DP / 16;      // steps of the first product; 16-byte pieces of a key
     constexpr int TD = DP / 32, NB = BK / 32, NG = BK / 16;
     constexpr int KP = DP * 2 + 16, VP = BK * 2 + 16;// bytes of a row in LDS
-    constexpr int K_TASKS = BK * NC, V_TASKS = BK / 4 * (DP / 4);
+    constexpr int NT = DP == 96 ? 8 : NC;          // as many lanes as have a key's pieces (of 96 columns some are idle: 6 would make a wavefront's keys lie in two pages)
+    constexpr int K_TASKS = BK * NT, V_TASKS = BK / 4 * (NT * 4);
     static_assert(K_TASKS == V_TASKS, "as many pieces of K as of V");
     constexpr int PER = (K_TASKS + kLanes - 1) / kLanes;// of a lane
     constexpr int TILES = 2 * (BK * KP + DP * VP), ROWS = kWaves * 32 * kRowPitch<DP>;
@@ -108,10 +109,10 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     const uint32_t my_tiles = some_see <= first_key ? 0 : (some_see - first_key + BK - 1) / BK < tiles ? (some_see - first_key + BK - 1) / BK : tiles;
 
     // a lane's pieces of a tile: 16 bytes of one key of K, 4 bytes of 4 keys of V
-    const auto k_key = [&](int i) { return (tid + i * kLanes) / NC; };
-    const auto k_piece = [&](int i) { return (tid + i * kLanes) % NC; };
-    const auto v_keys = [&](int i) { return (tid + i * kLanes) / (DP / 4) * 4; };
-    const auto v_col = [&](int i) { return (tid + i * kLanes) % (DP / 4) * 4; };
+    const auto k_key = [&](int i) { return (tid + i * kLanes) / NT; };
+    const auto k_piece = [&](int i) { return (tid + i * kLanes) % NT; };
+    const auto v_keys = [&](int i) { return (tid + i * kLanes) / (NT * 4) * 4; };
+    const auto v_col = [&](int i) { return (tid + i * kLanes) % (NT * 4) * 4; };
     const auto works = [&](int i) { return K_TASKS % kLanes == 0 || tid + i * kLanes < K_TASKS; };
     // (the 16 keys it is of: the same for the whole wavefront, for 16 keys are the pieces of whole wavefronts, or a
     // wavefront's pieces lie within 16 keys)
@@ -161,6 +162,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         for (int i = 0; i < PER; ++i) {
             if (!works(i)) continue;
             const uint8_t *p = k_base + lane_of64(k_group, tile % kAhead * NG + group_of(k_key(i)));
+            asm("" : "+v"(k_off[i]));// (not added to k_base before the loop: a scalar base and a 32-bit offset make one instruction)
             k_raw[i] = ld16(p + k_off[i]);
         }
     };
@@ -174,6 +176,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         for (int i = 0; i < PER; ++i) {
             if (!works(i)) continue;
             const uint8_t *p = v_base + lane_of64(v_group, tile % kAhead * NG + group_of(v_keys(i)));
+            asm("" : "+v"(v_off[i]));
 #pragma unroll
             for (int j = 0; j < 4; ++j, p += a.v_at.token) v_raw[i][j] = *reinterpret_cast<const uint32_t *>(p + v_off[i]);
         }
@@ -194,6 +197,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
                 to[w % 2 * 4 + 2] = y.x;
                 to[w % 2 * 4 + 3] = y.y;
             }
+            if (NT != NC && k_piece(i) >= NC) continue;
             *reinterpret_cast<f16x8 *>(k) = half[0];
             *reinterpret_cast<f16x8 *>(k + NC * 16) = half[1];
         }
@@ -221,6 +225,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             }
             // 16 keys in order of the accumulator's halves: 0-3, 8-11, 4-7, 12-15
             const uint32_t quad = v_keys(i) / 4 & 3u, place = (v_keys(i) & ~15u) + (quad & 1u) * 8 + (quad >> 1) * 4;
+            if (NT != NC && v_col(i) >= DP) continue;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const auto two = [&](int j) { return __builtin_bit_cast(uint32_t, c % 2 ? pair_of<FP8, true>(pair[j][c / 2]) : pair_of<FP8, false>(pair[j][c / 2])); };
@@ -503,8 +508,10 @@ void launch(const AttentionArgs &a, unsigned units, unsigned cut_tiles, hipStrea
 }
 template<bool FP8>
 void launch(const AttentionArgs &a, unsigned units, unsigned cut_tiles, hipStream_t s) {
-    switch (paged_dim(a.dim)) {
+    // (96, which the kernel for decoding does not have, saves a quarter of 128's products)
+    switch (a.dim > 64 && a.dim <= 96 ? 96 : paged_dim(a.dim)) {
         case 64: return launch<FP8, 64>(a, units, cut_tiles, s);
+        case 96: return launch<FP8, 96>(a, units, cut_tiles, s);
         case 128: return launch<FP8, 128>(a, units, cut_tiles, s);
         case 192: return launch<FP8, 192>(a, units, cut_tiles, s);
         default: return launch<FP8, 256>(a, units, cut_tiles, s);
