@@ -130,8 +130,13 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     // What tiles are loaded and computed with is read for 64 groups of 16 keys at once, one for each lane: the pages, ahead
     // for K and for V, and for the computation the scales.
     constexpr uint32_t kAhead = 64 / NG;// tiles of such a set
+    // (worked out where it is needed, which is seldom: before the loop it would take registers that the loop needs)
+    const auto seldom = [](uint32_t v) {
+        asm volatile("" : "+v"(v));
+        return v;
+    };
     const auto page_of = [&](uint32_t tile) {
-        const uint32_t key = first_key + tile * BK + lane * 16;
+        const uint32_t key = first_key + tile * BK + seldom(lane) * 16;
         if (key >= u.length) return -1;
         const int page = table[fast_quotient(key, a.rows.by_page)];
         return static_cast<uint32_t>(page) < a.pages ? page : -1;
@@ -145,19 +150,29 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     // where a group's first key is; no page: page 0, for any place will do
     const auto bytes_of = [&](uint32_t tile, int page, const PagedStrides &at) {
         return static_cast<uint64_t>(static_cast<int64_t>(page < 0 ? 0 : page) * at.page) +
-               static_cast<uint64_t>(place_of(first_key + tile * BK + lane * 16)) * at.token;
+               static_cast<uint64_t>(place_of(first_key + tile * BK + seldom(lane) * 16)) * at.token;
     };
-    uint64_t k_group, v_group, v_none;// v_none: a bit for each group without a page
+    uint64_t k_group, v_group, v_none, v_none_before;// v_none: a bit for each group without a page, of this set and the last
     {
         const int page = page_of(0);
         k_group = bytes_of(0, page, a.k_at);
         v_group = bytes_of(0, page, a.v_at);
-        v_none = __builtin_amdgcn_ballot_w64(page < 0);
+        v_none = v_none_before = __builtin_amdgcn_ballot_w64(page < 0);
     }
+    const auto k_set = [&](uint32_t tile) {
+        if (tile % kAhead == 0) k_group = bytes_of(tile, page_of(tile), a.k_at);
+    };
+    const auto v_set = [&](uint32_t tile) {
+        v_none_before = v_none;
+        if (tile % kAhead == 0) {
+            const int page = page_of(tile);
+            v_group = bytes_of(tile, page, a.v_at);
+            v_none = __builtin_amdgcn_ballot_w64(page < 0);
+        }
+    };
     u32x4 k_raw[PER];
     uint32_t v_raw[PER][4];
     const auto load_k = [&](uint32_t tile) {
-        if (tile % kAhead == 0 && tile != 0) k_group = bytes_of(tile, page_of(tile), a.k_at);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (!works(i)) continue;
@@ -167,11 +182,6 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         }
     };
     const auto load_v = [&](uint32_t tile) {
-        if (tile % kAhead == 0 && tile != 0) {
-            const int page = page_of(tile);
-            v_group = bytes_of(tile, page, a.v_at);
-            v_none = __builtin_amdgcn_ballot_w64(page < 0);
-        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (!works(i)) continue;
@@ -202,6 +212,12 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             *reinterpret_cast<f16x8 *>(k + NC * 16) = half[1];
         }
     };
+    // 4 keys of column c of a lane's: 16 keys lie in order of the accumulator's halves, 0-3, 8-11, 4-7, 12-15, and
+    // column d is row d / TD of the accumulator's tile d % TD
+    const auto v_place = [&](uint32_t tile, uint32_t keys, uint32_t col, int c) {
+        const uint32_t quad = keys / 4 & 3u, place = (keys & ~15u) + (quad & 1u) * 8 + (quad >> 1) * 4, d = col + c;
+        return v_lds(tile) + (d % TD * 32 + d / TD) * VP + place * 2;
+    };
     const auto store_v = [&](uint32_t tile) {// before the V of another tile is loaded
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -209,12 +225,6 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             uint32_t x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = v_raw[i][j];
-            // what lies behind the row's end, or in no page, may be anything: no number times 0 is 0
-            const bool none = (v_none >> (tile % kAhead * NG + group_of(v_keys(i))) & 1u) != 0;
-            if (none || first_key + tile * BK + BK > u.length) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = none || first_key + tile * BK + v_keys(i) + j >= u.length ? 0 : x[j];
-            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = prepare_codes<FP8>(x[j]);
             uint32_t pair[2][2];
@@ -223,15 +233,29 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
                 pair[j][0] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05010400u);
                 pair[j][1] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07030602u);
             }
-            // 16 keys in order of the accumulator's halves: 0-3, 8-11, 4-7, 12-15
-            const uint32_t quad = v_keys(i) / 4 & 3u, place = (v_keys(i) & ~15u) + (quad & 1u) * 8 + (quad >> 1) * 4;
             if (NT != NC && v_col(i) >= DP) continue;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const auto two = [&](int j) { return __builtin_bit_cast(uint32_t, c % 2 ? pair_of<FP8, true>(pair[j][c / 2]) : pair_of<FP8, false>(pair[j][c / 2])); };
-                // column d is row d / TD of the accumulator's tile d % TD
-                const uint32_t d = v_col(i) + c, row = d % TD * 32 + d / TD;
-                *reinterpret_cast<u32x2 *>(v_lds(tile) + row * VP + place * 2) = u32x2{two(0), two(1)};
+                *reinterpret_cast<u32x2 *>(v_place(tile, v_keys(i), v_col(i), c)) = u32x2{two(0), two(1)};
+            }
+        }
+    };
+    // What lies behind the row's end, or in no page, may be anything, and as e4m3 no number, which times 0 is not 0: a lane
+    // puts zeros where it has just stored it.
+    const auto clear_v = [&](uint32_t tile, uint64_t without) {
+        if (!FP8) return;
+        const uint32_t none = static_cast<uint32_t>(without >> (tile % kAhead * NG)) & ((1u << NG) - 1);
+        if (none == 0 && first_key + tile * BK + BK <= u.length) return;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t keys = seldom(v_keys(i)), col = seldom(v_col(i));
+            if (!works(i) || (NT != NC && col >= DP)) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if ((none >> group_of(v_keys(i)) & 1u) == 0 && first_key + tile * BK + keys + j < u.length) continue;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) *reinterpret_cast<uint16_t *>(v_place(tile, keys, col, c) + j * 2) = 0;
             }
         }
     };
@@ -287,7 +311,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         float v_log = -200.0f;
         k_scale = 0.0f;
         if (page >= 0) {
-            const uint32_t block = fast_quotient(place_of(first_key + tile * BK + lane * 16), a.by_block);
+            const uint32_t block = fast_quotient(place_of(first_key + tile * BK + seldom(lane) * 16), a.by_block);
             k_scale = ks_base[page * a.k_at.s_page + block];
             v_log = __builtin_amdgcn_logf(fmaxf(vs_base[page * a.v_at.s_page + block], 0x1p-126f));
         }
@@ -341,11 +365,12 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         const uint32_t key0 = first_key + tile * BK;
         const uint32_t none = static_cast<uint32_t>(no_page >> (tile % kAhead * NG)) & ((1u << NG) - 1);
         if (none != 0 || key0 + BK > all_see) {
+            const uint32_t mine = seldom(h * 4);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const uint32_t key = key0 + b * 32 + 8 * (i / 4) + 4 * h + i % 4;
+                    const uint32_t key = key0 + b * 32 + 8 * (i / 4) + mine + i % 4;
                     const bool gone = key >= limit || (none >> (2 * b + i / 8) & 1u) != 0;
                     s[b][i] = gone ? -__builtin_inff() : s[b][i];
                 }
@@ -373,6 +398,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         load_k(1);
         if (lead == 2) {
             store_v(0);
+            clear_v(0, v_none);
             load_v(1);
             store_k(1);
             load_k(2);
@@ -386,33 +412,38 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         __syncthreads();
         if (kTurns && wave >= 4) __syncthreads();
         for (uint32_t tile = 0; tile < tiles; ++tile) {
-            // (also behind the last tile, where nobody reads what is written: a condition here would make the compiler wait for
-            // all loads where the ways meet)
-            store_k(tile + lead);
-            store_v(tile + lead - 1);
-            load_k(tile + lead + 1);
-            load_v(tile + lead);
+            k_set(tile + lead + 1);
+            v_set(tile + lead);
+            // (also behind the last tile, where nobody reads what is written, and of tiles that none of these rows sees: a
+            // condition here would keep the rest from being mixed, and make the compiler wait for all loads where the ways meet)
             f16x8 p[NG];
-            if (tile < my_tiles) {
-                const uint32_t at = tile % kAhead * NG;
+            float sums = 0.0f;
+            const uint32_t now = tile % kAhead * NG;
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const float less = lane_of(v_rel, at + g) - m;
-                    float y[8], sum = 0.0f;
+            for (int g = 0; g < NG; ++g) {
+                const float less = lane_of(v_rel, now + g) - m;
+                float y[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + i], f[g], less));
-                        sum += y[i];
-                    }
-                    l = __builtin_fmaf(sum, lane_of(v_back, at + g), l);
+                for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + i], f[g], less));
+                sums = __builtin_fmaf(((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7])), lane_of(v_back, now + g), sums);
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const f16x2 w = __builtin_convertvector((f32x2{y[i], y[i + 1]}), f16x2);
-                        p[g][i] = w.x;
-                        p[g][i + 1] = w.y;
-                    }
+                for (int i = 0; i < 8; i += 2) {
+                    const f16x2 w = __builtin_convertvector((f32x2{y[i], y[i + 1]}), f16x2);
+                    p[g][i] = w.x;
+                    p[g][i + 1] = w.y;
+                }
+                if (g == NG / 2 - 1) {
+                    store_k(tile + lead);
+                    store_v(tile + lead - 1);
+                    load_k(tile + lead + 1);
+                    load_v(tile + lead);
                 }
             }
+            l = tile < my_tiles ? l + sums : l;
+            asm volatile("" : "+v"(l));// (not moved behind the barrier)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) asm volatile("" : "+v"(p[g]));
+            clear_v(tile + lead - 1, v_none_before);
             if (kTurns) __syncthreads();
             if (tile < my_tiles) {
                 // the next tile's products (behind the last they are not used), and this one's sums
