@@ -36,34 +36,34 @@ struct TileRows {
 template<int DP>
 constexpr int kRowPitch = DP * 2 + 16;
 
-template<int DP, typename F>
+template<int DP, int LANES = kWave, typename F>
 __device__ __forceinline__ void each_piece(const AttentionArgs &a, const TileRows &t, uint32_t lane, int64_t token_step, int64_t head_step, F f) {
     constexpr int PIECES = DP / 8;
 #pragma unroll
-    for (int j = 0; j < 32 * PIECES / kWave; ++j) {
-        const uint32_t index = lane + j * kWave, row = index / PIECES, piece = index % PIECES;
+    for (int j = 0; j < (32 * PIECES + LANES - 1) / LANES; ++j) {
+        const uint32_t index = lane + j * LANES, row = index / PIECES, piece = index % PIECES;
         const uint32_t r = t.row0 + row, token = fast_quotient(r, a.by_group);
         f(j, row < t.count && piece * 8 < a.dim, row * kRowPitch<DP> + piece * 16,
           static_cast<int64_t>(t.first + token) * token_step + static_cast<int64_t>(t.head * a.group + (r - token * a.group)) * head_step + piece * 8);
     }
 }
 
-// O times `by` to out, through LDS.  o[t][i] of lane (n, h) is column TD m' + t of row n, m' = 8 (i / 4) + 4 h + i % 4.
-template<int DP>
-__device__ __forceinline__ void put_rows(const AttentionArgs &a, const TileRows &rows, uint32_t lane, uint8_t *scratch, const f32x16 (&o)[DP / 32], float by) {
+// O times `by` into LDS, four of a lane's accumulators of each tile.  o[t][i] of lane (n, h) is column TD m' + t of
+// row n, m' = 8 (i / 4) + 4 h + i % 4.
+template<int DP, typename F>
+__device__ __forceinline__ void put_four(const AttentionArgs &a, uint32_t n32, uint32_t h, uint8_t *scratch, uint32_t i4, F o_by) {
     constexpr int TD = DP / 32;
-    const uint32_t n32 = lane & 31u, h = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-#pragma unroll
-        for (int c = 0; c < 4 * TD; c += 2) {// columns side by side
-            *reinterpret_cast<uint32_t *>(scratch + n32 * kRowPitch<DP> + ((2 * i + 4 * h) * TD + c) * 2) =
-                narrow2_rne(a.bf16, o[c % TD][i + c / TD] * by, o[(c + 1) % TD][i + (c + 1) / TD] * by);
-        }
+    for (int c = 0; c < 4 * TD; c += 2) {// columns side by side
+        *reinterpret_cast<uint32_t *>(scratch + n32 * kRowPitch<DP> + ((8 * i4 + 4 * h) * TD + c) * 2) =
+            narrow2_rne(a.bf16, o_by(c % TD, c / TD), o_by((c + 1) % TD, (c + 1) / TD));
     }
-    each_piece<DP>(a, rows, lane, a.out_token, a.out_head, [&](int, bool there, uint32_t in_lds, int64_t at) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(scratch + in_lds);
-        if (there) st16_any(a.out + at, w);
+}
+// Those rows to out.
+template<int DP, int LANES = kWave>
+__device__ __forceinline__ void put_rows(const AttentionArgs &a, const TileRows &rows, uint32_t lane, const uint8_t *scratch) {
+    each_piece<DP, LANES>(a, rows, lane, a.out_token, a.out_head, [&](int, bool there, uint32_t in_lds, int64_t at) {
+        if (there) st16_any(a.out + at, *reinterpret_cast<const u32x4 *>(scratch + in_lds));
     });
 }
 
@@ -491,51 +491,57 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             *reinterpret_cast<f32x4 *>(p + k * kWave) = f32x4{of(0), of(1), of(2), of(3)};
         }
     } else {
-        put_rows<DP>(a, my_rows, lane, scratch, o, l > 0.0f ? v_unit / l : 0.0f);
+        const float by = l > 0.0f ? v_unit / l : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) put_four<DP>(a, n32, h, scratch, i / 4, [&](int t, int j) { return o[t][i + j] * by; });
+        put_rows<DP>(a, my_rows, lane, scratch);
     }
 }
 
-// The units of a tile together, a wavefront for 32 query rows, in the lanes that held them.
+// The units of a tile together: 32 query rows a workgroup, in the lanes that held them, and a quarter of their sums a wavefront.
 template<int DP>
-__global__ __launch_bounds__(kWave) void paged_attention_tiles_join(AttentionArgs a) {
+__global__ __launch_bounds__(4 * kWave) void paged_attention_tiles_join(AttentionArgs a) {
     constexpr int TD = DP / 32;
     __shared__ __attribute__((aligned(16))) uint8_t scratch[32 * kRowPitch<DP>];
-    __shared__ uint64_t slots[1];
+    __shared__ uint64_t slots[4];
     __shared__ Unit shared_unit;
     Unit u;
-    const uint32_t waves = a.tile_rows / 32, wave = blockIdx.x % waves, head = blockIdx.x / waves % a.kv_heads;
-    if (!find_unit<1, true>(a, blockIdx.x / waves / a.kv_heads, slots, &shared_unit, &u)) return;
-    const uint32_t lane = threadIdx.x, n32 = lane & 31u;
-    const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens, rows = tokens * a.group, mine0 = u.tile * a.tile_rows + wave * 32;
+    const uint32_t waves = a.tile_rows / 32, part = blockIdx.x % waves, head = blockIdx.x / waves % a.kv_heads;
+    if (!find_unit<4, true>(a, blockIdx.x / waves / a.kv_heads, slots, &shared_unit, &u)) return;
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tid / kWave)));
+    const uint32_t n32 = lane & 31u;
+    const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens, rows = tokens * a.group, mine0 = u.tile * a.tile_rows + part * 32;
     if (mine0 >= rows) return;
-    const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * waves + wave; };
+    const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * waves + part; };
     float high = kNone;
+#pragma unroll 4
     for (uint32_t c = 0; c < u.chunks; ++c) high = fmaxf(high, a.part_stat[2 * (at(c) * 32 + n32)]);
-    f32x16 o[TD];
+    f32x4 o[TD];
 #pragma unroll
-    for (int t = 0; t < TD; ++t) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-    }
+    for (int t = 0; t < TD; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float total = 0.0f;
-#pragma unroll 1
+#pragma unroll 4
     for (uint32_t c = 0; c < u.chunks; ++c) {
-        f32x4 x[4 * TD];
-        const float *p = a.part_out + at(c) * (32 * DP) + lane * 4;
-#pragma unroll
-        for (int k = 0; k < 4 * TD; ++k) x[k] = ld16f(p + k * 4 * kWave);
+        const float *p = a.part_out + at(c) * (32 * DP) + wave * (4 * TD * kWave) + lane * 4;
         const float l = a.part_stat[2 * (at(c) * 32 + n32) + 1], by = __builtin_amdgcn_exp2f(a.part_stat[2 * (at(c) * 32 + n32)] - high);
         total += l * by;
 #pragma unroll
-        for (int k = 0; k < 16 * TD; ++k) o[k % TD][k / TD] += x[k / 4][k % 4] * by;
+        for (int k = 0; k < TD; ++k) {
+            const f32x4 x = ld16f(p + k * 4 * kWave);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[(k * 4 + j) % TD][(k * 4 + j) / TD] += x[j] * by;
+        }
     }
-    put_rows<DP>(a, TileRows{mine0, rows - mine0 < 32 ? rows - mine0 : 32, u.first, head}, lane, scratch, o, total > 0.0f ? 1.0f / total : 0.0f);
+    const float by = total > 0.0f ? 1.0f / total : 0.0f;
+    put_four<DP>(a, n32, lane >> 5, scratch, wave, [&](int t, int j) { return o[t][j] * by; });
+    __syncthreads();
+    put_rows<DP, 4 * kWave>(a, TileRows{mine0, rows - mine0 < 32 ? rows - mine0 : 32, u.first, head}, tid, scratch);
 }
 
 template<bool FP8, int DP>
 void launch(const AttentionArgs &a, unsigned units, unsigned cut_tiles, hipStream_t s) {
     paged_attention_tiles<FP8, DP><<<units, paged_tile_waves(DP) * kWave, 0, s>>>(a);
-    paged_attention_tiles_join<DP><<<cut_tiles * paged_tile_waves(DP), kWave, 0, s>>>(a);
+    paged_attention_tiles_join<DP><<<cut_tiles * paged_tile_waves(DP), 4 * kWave, 0, s>>>(a);
 }
 template<bool FP8>
 void launch(const AttentionArgs &a, unsigned units, unsigned cut_tiles, hipStream_t s) {
