@@ -49,31 +49,40 @@ __device__ __forceinline__ RowWork row_work(const AttentionArgs &a, const RowSpa
     return RowWork{fast_quotient(rows + a.tile_rows - 1, a.by_tile), (s.length + kStepKeys - 1) / kStepKeys};
 }
 
-// How many units a row's tiles are cut into where a unit has up to `steps`.
+// How many units a row's tiles are cut into where a unit has up to `steps`, and how many steps the longest then has.
 __device__ __forceinline__ uint32_t unit_chunks(const RowWork &w, uint32_t steps) { return w.steps > steps ? (w.steps + steps - 1) / steps : 1u; }
+
+__device__ __forceinline__ uint32_t unit_longest(const AttentionArgs &a, const RowWork &w, uint32_t chunks) {
+    return ((w.steps + chunks - 1) / chunks + a.whole_steps - 1) & ~(a.whole_steps - 1);
+}
+// All rows' units, and the longest's steps.
+struct UnitSum {
+    float units, longest;
+};
 
 // Steps of a unit, from the work of all rows.  Cut into `target` parts, rows of unequal length leave odd ends.  Where
 // many more workgroups wait than run (a.rounds_each is 0) these even out.  Otherwise the GPU takes the units in rounds,
-// and of target, 3/2, 2 and 3 times as many parts those are taken whose rounds are the shortest together (a unit's
-// beginning and end are worth 4 steps).  count(steps): units of all rows.
+// and of 2/3 to 3 times target parts those are taken whose rounds are the shortest together (a unit's
+// beginning and end are worth 4 steps; 2505 query rows beside 8 of single ones: 3 units a tile in one round 243 us, 5 in two 275).
+// sum(steps): of all rows.
 template<typename F>
-__device__ __forceinline__ uint32_t unit_steps(const AttentionArgs &a, float total, F count) {
+__device__ __forceinline__ uint32_t unit_steps(const AttentionArgs &a, float total, F sum) {
     const auto cut = [&](float by) {
         // at least total / target, with room for the roundings on the way
         uint32_t steps = static_cast<uint32_t>(total * a.units_each * by * 1.00001f) + 1;
         steps = steps < a.least_steps ? a.least_steps : steps > 0x40000000u ? 0x40000000u : steps;
         return (steps + a.whole_steps - 1) & ~(a.whole_steps - 1);
     };
-    uint32_t best = cut(1.0f);
-    if (a.rounds_each == 0.0f) return best;
+    if (a.rounds_each == 0.0f) return cut(1.0f);
     float least = __builtin_inff();
-    uint32_t last = 0;
+    uint32_t best = 0, last = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t steps = cut(i == 0 ? 1.0f : i == 1 ? 2.0f / 3 : i == 2 ? 0.5f : 1.0f / 3);
+    for (int i = 0; i < 6; ++i) {
+        const uint32_t steps = cut(i == 0 ? 1.5f : i == 1 ? 1.25f : i == 2 ? 1.0f : i == 3 ? 2.0f / 3 : i == 4 ? 0.5f : 1.0f / 3);
         if (steps == last) break;// (the least there may be)
         last = steps;
-        const float time = ceilf(count(steps) * a.rounds_each) * static_cast<float>(steps + 4);
+        const UnitSum all = sum(steps);
+        const float time = ceilf(all.units * a.rounds_each) * (all.longest + 4.0f);
         if (time < least) {
             least = time;
             best = steps;
@@ -88,7 +97,7 @@ __device__ __forceinline__ Unit unit_of(const AttentionArgs &a, uint32_t r, cons
     const uint32_t nth = JOIN ? i : i / chunks;
     // a prompt's last tiles see the most keys and begin first
     return Unit{r, w.tiles - 1 - nth, JOIN ? 0 : i - nth * chunks, chunks, s.first, s.count, s.length,
-                ((w.steps + chunks - 1) / chunks + a.whole_steps - 1) & ~(a.whole_steps - 1), slot + nth * chunks};
+                unit_longest(a, w, chunks), slot + nth * chunks};
 }
 
 // Unit number `index` of all (JOIN: tile number `index` of those that have several units); false if there are fewer.
@@ -102,7 +111,11 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, uint32_t index
         if (lane < a.rows.rows) s = row_span(a.rows, lane);
         const RowWork w = row_work(a, s);
         const uint32_t steps = unit_steps(a, wave_sum(static_cast<float>(w.tiles) * static_cast<float>(w.steps)),
-                                          [&](uint32_t n) { return wave_sum(static_cast<float>(w.tiles * unit_chunks(w, n))); });
+                                          [&](uint32_t n) {
+                                              const uint32_t chunks = unit_chunks(w, n);
+                                              return UnitSum{wave_sum(static_cast<float>(w.tiles * chunks)),
+                                                             wave_max(w.tiles == 0 ? 0.0f : static_cast<float>(unit_longest(a, w, chunks)))};
+                                          });
         const uint32_t chunks = unit_chunks(w, steps), units = w.tiles * chunks, mine = JOIN ? (chunks > 1 ? w.tiles : 0) : units;
         const uint32_t end = wave_scan(mine), in_slots = chunks > 1 ? units : 0, slot = wave_scan(in_slots) - in_slots;
         const uint64_t hit = __builtin_amdgcn_ballot_w64(index < end && index >= end - mine);
@@ -124,12 +137,15 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, uint32_t index
     block_scan64<WAVES>(work, slots, &total);
     const uint32_t steps = unit_steps(a, static_cast<float>(total), [&](uint32_t n) {
         uint64_t units = 0, sum;
+        float longest = 0.0f;
         for (uint32_t r = r0; r < r1; ++r) {
             const RowWork w = row_work(a, row_span(a.rows, r));
-            units += static_cast<uint64_t>(w.tiles) * unit_chunks(w, n);
+            const uint32_t chunks = unit_chunks(w, n);
+            units += static_cast<uint64_t>(w.tiles) * chunks;
+            if (w.tiles != 0) longest = fmaxf(longest, static_cast<float>(unit_longest(a, w, chunks)));
         }
         block_scan64<WAVES>(units, slots, &sum);
-        return static_cast<float>(sum);
+        return UnitSum{static_cast<float>(sum), block_max<WAVES>(longest, slots)};
     });
     // low half: units (JOIN: tiles of several), high half: slots of the workspace
     const auto counts = [&](const RowWork &w, uint32_t chunks) {

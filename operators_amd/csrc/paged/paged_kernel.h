@@ -87,6 +87,19 @@ __device__ __forceinline__ uint64_t block_scan64(uint64_t v, uint64_t *slots, ui
     return before + sum - v;
 }
 
+// The largest of all lanes' values, which are not below 0.
+template<int WAVES>
+__device__ __forceinline__ float block_max(float v, uint64_t *slots) {
+    v = wave_max(v);
+    if ((threadIdx.x & (kWave - 1)) == 0) slots[threadIdx.x / kWave] = __float_as_uint(v);
+    __syncthreads();
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) top = fmaxf(top, __uint_as_float(static_cast<uint32_t>(slots[i])));
+    __syncthreads();
+    return top;
+}
+
 // ---- codes as fp16 ------------------------------------------------------------
 // Both types are exact in fp16: whole numbers up to 128, and e4m3.
 // An int8 with its sign bit turned over, as the low byte of 0x64xx, is the fp16
