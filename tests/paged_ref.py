@@ -112,11 +112,15 @@ def attention_bound(want, mean, size, dtype, dim, length, v_top):
         A weight changes by twice that (its own and the sum's);
       * a weight too small for fp16's normal numbers, which is held 2^10 up: half a step of 2^-24 there, 2^-35 of the largest weight
         and so of their sum, times the largest value (code times the row's largest V scale, `v_top`), for each key;
+      * prompts: a V scale goes into the exponent as its log2, relative to the largest one's.  The log2 is at most 126, so it and the two sums it
+        goes through are off by at most a step and two halves of 2^-17, 2^-16 in the exponent, and the value by ln 2 of that: 2^-16 of
+        the mean.  (It is taken out of the weights' own sum with the same error.)  A scale 2^-40 times smaller than the largest has
+        weights that fp16 holds as 0: that is within the last point's 2^-35;
       * sums over keys in fp32: one rounding for each 32 keys and each joined part, 2^-24 of the mean each."""
     delta = (dim + 16) * 2.0 ** -24 * size + 2.0 ** -22 * (1 + size)
     eps = torch.finfo(FLOAT[dtype]).eps / 2
     tiny = torch.finfo(FLOAT[dtype]).tiny * torch.finfo(FLOAT[dtype]).eps
-    inside = 2.0 ** -35 * length * v_top + (2.0 ** -11 + 2.0 ** -24 * (length / 32 + 600)) * mean + 2 * delta[..., None] * mean
+    inside = 2.0 ** -35 * length * v_top + (2.0 ** -11 + 2.0 ** -16 + 2.0 ** -24 * (length / 32 + 600)) * mean + 2 * delta[..., None] * mean
     return inside + eps * (want.abs() + inside) + tiny
 
 
