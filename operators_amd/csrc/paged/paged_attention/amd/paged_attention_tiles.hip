@@ -3,17 +3,23 @@
 // A workgroup takes 256 query rows of one K/V head (tokens by heads of its group), a
 // wavefront 32 of them, and all walk the keys together, 64 at a time (heads wider than
 // 128: 128 rows, for one wavefront's registers are two's, and 32 keys).  A tile's codes
-// are turned into fp16 once for all wavefronts on their way into LDS, keys by columns for K, columns by keys for V, so that either
-// product reads its operand as 16-byte vectors; rows are 16 bytes longer than a power
-// of two, which spreads eight neighbouring lanes over all banks.  Two tiles lie in LDS:
-// while one is computed with, the next is written and the one behind it is on its way
-// from memory; one barrier a tile.
+// are turned into fp16 once for all wavefronts on their way into LDS, keys by columns
+// for K, columns by keys for V, so that either product reads its operand as 16-byte
+// vectors; rows are 16 bytes longer than a power of two, which spreads eight
+// neighbouring lanes over all banks.  Two tiles lie in LDS: while one is computed with,
+// the next is written and the one behind it is on its way from memory.
 // v_mfma_f32_32x32x16 leaves a lane 16 of the 32 keys of one query, and V's keys lie in
 // the order in which those make up the second product's operand, so P is not exchanged.
 // The V scale of a block is added to the exponent (P = exp2(x - m + log2 r)) and taken
 // out of its sum again (sum / r), which saves a product for each score.
-// Bound by the matrix units and, nearly as much, by the vector units (about 7 slots for
-// each score, 4 of them the exponential) and LDS (both operands for 32 rows a wavefront).
+// Two wavefronts share a SIMD and are a phase apart: one at its products, the other at
+// its exponentials and the next tile's codes (without that 353 us below, with wavefronts
+// of the same phase on a SIMD 390).  64 heads on 8 of 128 columns, a prompt of 4096 tokens:
+// 309-318 us, 0.88 PFLOP/s; a library product of large fp16 matrices reaches 1.34.  Of that
+// time the matrix units are at work 40 %, the vector units 55 % (7 slots for each
+// score, 4 of them the exponential); LDS hands on 128 bytes a clock in each phase of
+// products, all that it can, for 32 rows a wavefront read either operand anew.
+// Two wavefronts of 64 rows would halve that, but not fit into the registers.
 #include "paged_attention_units.h"
 
 namespace {
@@ -432,13 +438,11 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
                     p[g][i] = w.x;
                     p[g][i + 1] = w.y;
                 }
-                if (g == NG / 2 - 1) {
-                    store_k(tile + lead);
-                    store_v(tile + lead - 1);
-                    load_k(tile + lead + 1);
-                    load_v(tile + lead);
-                }
             }
+            store_k(tile + lead);
+            store_v(tile + lead - 1);
+            load_k(tile + lead + 1);
+            load_v(tile + lead);
             l = tile < my_tiles ? l + sums : l;
             asm volatile("" : "+v"(l));// (not moved behind the barrier)
 #pragma unroll
