@@ -13,13 +13,15 @@
 // The V scale of a block is added to the exponent (P = exp2(x - m + log2 r)) and taken
 // out of its sum again (sum / r), which saves a product for each score.
 // Two wavefronts share a SIMD and are a phase apart: one at its products, the other at
-// its exponentials and the next tile's codes (without that 353 us below, with wavefronts
-// of the same phase on a SIMD 390).  64 heads on 8 of 128 columns, a prompt of 4096 tokens:
-// 309-318 us, 0.88 PFLOP/s; a library product of large fp16 matrices reaches 1.34.  Of that
-// time the matrix units are at work 40 %, the vector units 55 % (7 slots for each
-// score, 4 of them the exponential); LDS hands on 128 bytes a clock in each phase of
-// products, all that it can, for 32 rows a wavefront read either operand anew.
-// Two wavefronts of 64 rows would halve that, but not fit into the registers.
+// its exponentials and the next tile's codes (when that took 330 us in the example
+// below: 353 without, 390 with wavefronts of the same phase on a SIMD).
+// 64 heads on 8 of 128 columns, a prompt of 4096 tokens: 309-318 us, 0.88 PFLOP/s; a
+// library product of large fp16 matrices reaches 1.34.  Of that time the matrix units
+// are at work 40 %, the vector units 55 % (7 slots for each score, 4 of them the
+// exponential); LDS hands on 128 bytes a clock in each phase of products, all that it
+// can, for 32 rows a wavefront read either operand anew.  Two wavefronts of 64 rows
+// would halve that, but not fit into the registers.  Heads of 256 columns, 32 on 8, 2048
+// tokens: 168 us, 0.41 PFLOP/s, for one wavefront a SIMD overlaps nothing.
 #include "paged_attention_units.h"
 
 namespace {

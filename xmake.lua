@@ -1,4 +1,4 @@
--- xmake build of libinfiniop.so with the amd-gpu device (AMD Instinct MI355X, gfx950 only).
+-- xmake build of libinfiniop.so and libinfiniop_paged.so with the amd-gpu device (AMD Instinct MI355X, gfx950 only).
 --
 --     xmake f --amd-gpu=y && xmake && xmake install      -- into $INFINI_ROOT (default ~/.infini)
 --
@@ -76,6 +76,15 @@ if has_config("amd-gpu") then
         add_files(CSRC .. "/ops/*/amd/*.hip", {rules = "hipcc"})
     target_end()
 
+    target("amd-gpu-paged")
+        set_kind("static")
+        on_install(function (target) end)
+        set_languages("cxx17")
+        add_includedirs("include")
+        add_files(CSRC .. "/paged/*/amd/*.cc", {rules = "hipcc"})
+        add_files(CSRC .. "/paged/*/amd/*.hip", {rules = "hipcc"})
+    target_end()
+
 end
 
 target("infiniop")
@@ -98,4 +107,22 @@ target("infiniop")
     set_installdir(os.getenv("INFINI_ROOT") or (os.getenv("HOME") .. "/.infini"))
     add_installfiles("include/(**/*.h)", {prefixdir = "include"})
     add_installfiles("include/*.h", {prefixdir = "include"})
+target_end()
+
+-- the operators of the paged cache, which the reference does not have; on handles and descriptors of libinfiniop.so
+target("infiniop_paged")
+    set_kind("shared")
+    if has_config("amd-gpu") then
+        add_deps("amd-gpu-paged")
+    end
+    set_languages("cxx17")
+    set_toolset("ld", HIPCC)
+    set_toolset("sh", HIPCC)
+    add_shflags("--offload-arch=gfx950", {force = true})
+    add_includedirs(ROCM .. "/include")
+    add_defines("__HIP_PLATFORM_AMD__")
+    add_cxxflags("-fPIC", "-fvisibility=hidden")
+    add_files(CSRC .. "/paged/*/operator.cc")
+
+    set_installdir(os.getenv("INFINI_ROOT") or (os.getenv("HOME") .. "/.infini"))
 target_end()
