@@ -5,8 +5,9 @@
 
 namespace {
 
-// Sequences of up to this many query rows go to the kernel for decoding.
-constexpr uint32_t kFewRows = 32;
+// Sequences of up to this many query rows go to the kernel for decoding, in tiles of 32 that each read the keys (us, 64/8 heads x 128,
+// there and with the kernel for prompts: 64 rows of 32 x 8192 keys 195 and 246, of 8 x 800 22.6 and 29.7; 96 rows of 32 x 8192 280 and 251).
+constexpr uint32_t kFewRows = 64;
 
 // Only tiles of several units use the workspace: of those, a tile of k keys is cut at every c of them where the sum of
 // all k is at most (most_units - most_tiles) * c, so they are at most twice that many of a head (ceil(x) <= 2 x from 1 on).
