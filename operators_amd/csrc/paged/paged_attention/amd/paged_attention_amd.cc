@@ -63,8 +63,9 @@ infiniopStatus_t amdCreatePagedAttentionDescriptor(AmdHandle_t handle, PagedAtte
     // (one sequence that may have many query rows goes to the kernel for prompts whatever it has: one launch less)
     few.most_tiles = busy == 1 && most_rows > kFewRows ? 0 : static_cast<uint32_t>(query_rows / few.tile_rows + busy);
     // as many units as the GPU holds, twice that where rows of unequal length meet (us, bf16, 64/8 heads x 128: 48 rows of
-    // 100 to 131072 tokens 389 and 353, 32 of 8192 95 and 96; one of 131072 53 and 56)
-    few.target = static_cast<uint32_t>(amd::ceil_div((rows.rows == 1 ? 2 : 4) * cus, cache.kv_heads));
+    // 100 to 131072 tokens 389 and 353, 32 of 8192 95 and 96; one of 131072 53 and 56); of 256 columns it holds one workgroup
+    // a compute unit (32 rows of 100 to 32768 tokens 176 with twice the compute units, 182 with four times; of 8192 190 and 211)
+    few.target = static_cast<uint32_t>(amd::ceil_div((rows.rows == 1 || paged_dim(cache.dim) == 256 ? 2 : 4) * cus, cache.kv_heads));
     few.most_units = few.target + few.most_tiles;
     many.tile_rows = 32 * paged_tile_waves(paged_dim(cache.dim));
     many.least = busy == 1 ? 1 : kFewRows + 1;
