@@ -289,3 +289,22 @@ def test_random_problems(ctx):
                     cache=rng.choice(["i8", "e4m3"]), dtype=rng.choice(["f16", "bf16"]), layout=rng.choice(["dense", "tokens first", "wide"]), seed=trial)
         print(trial, p.rows, p.heads, p.kv, p.dim, p.page, p.cache, p.dtype, flush=True)
         p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("dim", [80, 128, 256])
+@pytest.mark.parametrize("new", [4, 5, 8, 9, 16, 17])
+def test_between_decoding_and_prompts(ctx, new, dim):
+    """32, 40, 64, 72, 128 and 136 query rows of a K/V head, one sequence long enough to be shared, beside single tokens and longer chunks."""
+    for rows in ([(3000, new), (10, new), (700, 1), (0, new)], [(5000, new)], [(900, new), (40, 90), (0, 1)]):
+        p = Problem(rows, heads=8, kv_heads=1, dim=dim, cache="e4m3", dtype="bf16", seed=new + dim)
+        p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [80, 96, 112, 192, 256])
+def test_prompts_past_missing_pages(ctx, dim, cache):
+    """Pages that are none inside a chunk's keys, in every width that tiles are held in, with page sizes that end inside a tile of 64 keys."""
+    for page in (16, 48, 80):
+        p = Problem([(300, 131), (5, 77), (0, 200)], heads=4, kv_heads=2, dim=dim, page=page, cache=cache, dtype="f16", seed=dim + page)
+        p.table[0, 1], p.table[0, 3], p.table[2, 0] = -1, 10 ** 6, -7
+        p.check(p.run(ctx))
