@@ -20,7 +20,7 @@
 // exchange between lanes.
 // Bound by reading K and V once from HBM: 64 heads on 8 of 128 columns, 48 sequences of
 // 100 to 131072 keys 347 us (5.5 TB/s; a large element-wise pass reaches 6.2), one of 131072
-// 52 us (5.1), one of 1000 11.4 us, which is two launches and four waits for memory in turn.
+// 52 us (5.1), one of 1000 10.7 us, which is two launches and four waits for memory in turn.
 #include "paged_attention_units.h"
 
 namespace {
