@@ -308,3 +308,48 @@ def test_prompts_past_missing_pages(ctx, dim, cache):
         p = Problem([(300, 131), (5, 77), (0, 200)], heads=4, kv_heads=2, dim=dim, page=page, cache=cache, dtype="f16", seed=dim + page)
         p.table[0, 1], p.table[0, 3], p.table[2, 0] = -1, 10 ** 6, -7
         p.check(p.run(ctx))
+
+
+# ---- more than 64 rows: the units are found by a scan over the workgroup ------------
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("count", [65, 257, 300])
+def test_many_rows_some_shared_by_workgroups(ctx, count, cache):
+    rows = [((37 * r) % 90, 0 if r % 13 == 5 else 1) for r in range(count)]
+    rows[3], rows[40], rows[count - 1] = (6000, 1), (2500, 2), (9000, 1)
+    p = Problem(rows, heads=8, kv_heads=1, dim=64, page=64, block=16, cache=cache, dtype="bf16", seed=count)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("count, dim", [(65, 64), (300, 80), (600, 64), (300, 256)])
+def test_many_rows_with_chunks(ctx, count, dim, cache):
+    """Chunks of more than 64 query rows among them, long enough to be cut, with both kernels and both joins."""
+    rows = [((37 * r) % 90, 0 if r % 13 == 5 else 1) for r in range(count)]
+    rows[0], rows[30], rows[50], rows[count - 2] = (3000, 70), (0, 90), (4000, 1), (1500, 33)
+    p = Problem(rows, heads=4, kv_heads=1, dim=dim, page=32, block=32, cache=cache, dtype="f16", seed=count + dim)
+    p.check(p.run(ctx))
+
+
+def test_many_rows_replayed_with_other_lengths(ctx):
+    from operators_amd.ops import PagedAttentionPlan
+
+    rows = [((37 * r) % 90, 1) for r in range(130)]
+    rows[7], rows[100] = (5000, 1), (700, 40)
+    p = Problem(rows, heads=4, kv_heads=2, dim=64, cache="e4m3", dtype="bf16", seed=1, garbage=False)
+    kc, vc, ks, vs, table, offsets, lengths = p.args()
+    q, out = p.q.to(DEV), torch.full_like(p.q, 77.0, device=DEV)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with PagedAttentionPlan(ctx, out, q, kc, vc, ks, vs, table, offsets, lengths, 40, p.scale) as plan:
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            plan(out, q, kc, vc, ks, vs, table, offsets, lengths, stream=torch.cuda.current_stream().cuda_stream)
+        full = list(rows)
+        for cut in (0, 600, 4500, 0):
+            p.rows = [(max(0, had - cut) if had > 90 else had, new) for had, new in full]
+            p.lengths = torch.tensor([a + b for a, b in p.rows], dtype=torch.int32)
+            lengths.copy_(p.lengths)
+            out.fill_(77.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            p.check(out)

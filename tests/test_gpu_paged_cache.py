@@ -233,6 +233,21 @@ def test_append_of_nothing(ctx):
     ctx.kv_cache_append(codes, codes, scales, scales, one, one, torch.zeros(0, 1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), none)
 
 
+def test_append_many_rows_of_several_tokens(ctx):
+    # more than two tokens a row and more rows than a workgroup has lanes: units are found by a scan, several rows a lane
+    rows = [((7 * r) % 50, (0 if r % 5 == 2 else 3 + (r % 29 == 0) * 40)) for r in range(300)]
+    assert sum(b for _, b in rows) > 2 * len(rows)
+    check_append(ctx, rows, cache="e4m3", dim=16, heads=1, page=16)
+    check_append(ctx, rows, cache="i8", dim=32, heads=3, page=32, block=32, dtype="bf16", behind=7)
+
+
+def test_append_more_than_1024_rows(ctx):
+    # plain decoding of more rows than a token's row is looked up among
+    rows = [((7 * r) % 50, 0 if r % 11 == 3 else 1) for r in range(1100)]
+    check_append(ctx, rows, cache="e4m3", dim=16, heads=1, page=16)
+    check_append(ctx, [((3 * r) % 20, 0 if r % 2 else 2) for r in range(1100)], cache="i8", dim=16, heads=1, page=16, dtype="bf16")
+
+
 # ---- KVCacheCopy ---------------------------------------------------------------
 @pytest.mark.parametrize("layout", ["dense", "tokens first", "wide"])
 @pytest.mark.parametrize("dim, heads, page, block, pages", [(16, 1, 16, 16, 5), (80, 3, 48, 16, 9), (128, 8, 64, 32, 20), (256, 2, 128, 128, 6)])
