@@ -10,14 +10,17 @@
 // Codes are exact in fp16; q is multiplied by a power of two for each row that
 // brings its largest element to [1, 2), so that it is too (but for what is 2^24 times
 // smaller than that element), whatever its type.  Scores, maxima, sums and O are fp32.
-// P in fp16 costs each weight at most 2^-11 of itself, as much as rounding `out` to
-// fp16 does and an eighth of bf16; the scale of a V block goes into P, relative to
-// the largest one so far.  P is lifted by 2^10, so that of a weight too small for
-// that at most 2^-35 of the largest is lost, and the sum of very many small weights
-// beside a large one is kept: m is the maximum less 10.
-// The maximum is moved only when a score exceeds it by 2^4, and the V scale when one
-// is over twice as large (P stays below 2^15), which leaves the usual step without an
-// exchange between lanes.
+// The scale of a V block goes into P, whose running maximum is its own: with m_o of
+// score + log2(V scale) and m of the scores,
+//     P = exp2(score + log2(V scale) - m_o),  l = sum(exp2(score - m)),  out = V^T P 2^(m_o - m) / l
+// so that what fp16 holds of P depends on nothing but what the query row sees and gives
+// weight to, and neither O nor l on how large the values are.  P in fp16 costs each of
+// these products at most 2^-11 of itself, as much as rounding `out` to fp16 does and an
+// eighth of bf16.  It is lifted by 2^10, so that of one too small for that at most 2^-35 of
+// the row's largest is lost, and the sum of very many small ones beside a large one is
+// kept: m and m_o are the maxima less 10.
+// The maxima are moved only when one is exceeded by 2^4 (P stays below 2^15), which
+// leaves the usual step without an exchange between lanes.
 // Bound by reading K and V once from HBM: 64 heads on 8 of 128 columns, 48 sequences of
 // 100 to 131072 keys 347 us (5.5 TB/s; a large element-wise pass reaches 6.2), one of 131072
 // 52 us (5.1), one of 1000 10.7 us, which is two launches and four waits for memory in turn.
@@ -28,9 +31,10 @@ namespace {
 using namespace amd;
 
 constexpr int kWaves = 4;
-constexpr float kLift = 10.0f;   // log2 of P where the score is the running maximum
-constexpr float kSlack = 4.0f;   // log2 by which a score may exceed the running maximum
+constexpr float kLift = 10.0f;   // log2 of P where it is the running maximum
+constexpr float kSlack = 4.0f;   // log2 by which the running maximum may be exceeded
 constexpr float kNone = -1.0e30f;// the maximum of no score
+constexpr float kFar = 100.0f;   // log2 up to which P is exp2(score - m) times a power: what that loses below 2^-126 is nothing in fp16
 
 // maximum and sum over the four lanes that hold one query row
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
@@ -78,7 +82,7 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
     constexpr int KS = DP / 32, CH = DP / 64, VB = DP / 16, WORDS = DP / 64;
     __shared__ uint64_t slots[kWaves];
     __shared__ Unit shared_unit;
-    __shared__ float stat[2][kWaves][16 * NT];
+    __shared__ float stat[3][kWaves][16 * NT];
     __shared__ f32x4 meet[2][NT * VB][kWave];
     Unit u;
     const uint32_t head = blockIdx.x % a.kv_heads;
@@ -107,10 +111,10 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
     // steps s0 + wave, + 4, ...: page and scales of 32 of them are read at once, a half step by each lane;
     // the first of these are on their way while the queries are made ready
     int page = -1;
-    float k_scale = 0.0f, v_scale = 0.0f;
+    float k_scale = 0.0f, v_log = 0.0f;
     const auto groups = [&](uint32_t base) {
         page = -1;
-        k_scale = v_scale = 0.0f;
+        k_scale = v_log = 0.0f;
         const uint32_t key = ((base + kWaves * (lane >> 1)) * 2 + (lane & 1)) * 16;
         if (key < u.length && base + kWaves * (lane >> 1) < s1) {
             const uint32_t col = fast_quotient(key, a.rows.by_page);
@@ -118,7 +122,7 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
             if (static_cast<uint32_t>(page) < a.pages) {
                 const uint32_t block = fast_quotient(key - col * a.rows.page, a.by_block);
                 k_scale = ks_base[page * a.k_at.s_page + block];
-                v_scale = vs_base[page * a.v_at.s_page + block];
+                v_log = log2_of(vs_base[page * a.v_at.s_page + block]);
             } else {
                 page = -1;
             }
@@ -166,15 +170,14 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
     }
 
     f32x4 o[NT][VB];
-    float m[NT], l[NT];
+    float m[NT], l[NT], mo[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        m[t] = kNone;
+        m[t] = mo[t] = kNone;
         l[t] = 0.0f;
 #pragma unroll
         for (int j = 0; j < VB; ++j) o[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    float v_top = 0.0f, v_inv = 0.0f;// the largest V scale that O stands relative to, and its inverse
 
     for (uint32_t base = s0 + wave; base < s1; base += kWaves * 32) {
         if (base != s0 + wave) groups(base);
@@ -211,8 +214,8 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
             const int pg0 = __builtin_amdgcn_readlane(page, 2 * i), pg1 = __builtin_amdgcn_readlane(page, 2 * i + 1);
             const float ks[2] = {__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, k_scale), 2 * i)),
                                  __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, k_scale), 2 * i + 1))};
-            const float vs[2] = {__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v_scale), 2 * i)),
-                                 __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v_scale), 2 * i + 1))};
+            const float vl[2] = {__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v_log), 2 * i)),
+                                 __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v_log), 2 * i + 1))};
             f32x4 s[NT][2];
 #pragma unroll
             for (int t2 = 0; t2 < NT; ++t2) s[t2][0] = s[t2][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -242,18 +245,6 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
                     }
                 }
             }
-            const float v_now = fmaxf(vs[0], vs[1]);
-            if (v_now > 2.0f * v_top) {
-                // (never below 2^-100, whose inverse is far from infinity)
-                const float next = fmaxf(v_now, 0x1p-100f), by = v_top / next;
-                v_top = next;
-                v_inv = 1.0f / next;
-#pragma unroll
-                for (int t2 = 0; t2 < NT; ++t2) {
-#pragma unroll
-                    for (int j = 0; j < VB; ++j) o[t2][j] *= by;
-                }
-            }
             f16x8 p[NT];
 #pragma unroll
             for (int t2 = 0; t2 < NT; ++t2) {
@@ -271,26 +262,34 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
                         x[i2] = gone ? -__builtin_inff() : x[i2];
                     }
                 }
-                float high = x[0];
-#pragma unroll
-                for (int i2 = 1; i2 < 8; ++i2) high = fmaxf(high, x[i2]);
-                if (__builtin_amdgcn_ballot_w64(high > m[t2] + (kLift + kSlack)) != 0) {
-                    const float next = fmaxf(m[t2], quad_max(high) - kLift), by = __builtin_amdgcn_exp2f(m[t2] - next);
+                const float high0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), high1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]));
+                const float high = fmaxf(high0, high1), high_o = fmaxf(high0 + vl[0], high1 + vl[1]);
+                if (__builtin_amdgcn_ballot_w64(high > m[t2] + (kLift + kSlack) || high_o > mo[t2] + (kLift + kSlack)) != 0) {
+                    const float next = fmaxf(m[t2], quad_max(high) - kLift), next_o = fmaxf(mo[t2], quad_max(high_o) - kLift);
+                    l[t2] *= __builtin_amdgcn_exp2f(m[t2] - next);
+                    const float by = __builtin_amdgcn_exp2f(mo[t2] - next_o);
                     m[t2] = next;
-                    l[t2] *= by;
+                    mo[t2] = next_o;
 #pragma unroll
                     for (int j = 0; j < VB; ++j) o[t2][j] *= by;
                 }
                 float sum = 0.0f;
-                const float r0 = vs[0] * v_inv, r1 = vs[1] * v_inv;
                 float y[8];
 #pragma unroll
                 for (int i2 = 0; i2 < 8; ++i2) {
                     y[i2] = __builtin_amdgcn_exp2f(x[i2] - m[t2]);
                     sum += y[i2];
-                    y[i2] *= i2 < 4 ? r0 : r1;
                 }
                 l[t2] += sum;
+                const float r0 = vl[0] + (m[t2] - mo[t2]), r1 = vl[1] + (m[t2] - mo[t2]);
+                if (__builtin_amdgcn_ballot_w64(fmaxf(r0, r1) > kFar) != 0) {
+#pragma unroll
+                    for (int i2 = 0; i2 < 8; ++i2) y[i2] = __builtin_amdgcn_exp2f(x[i2] + (vl[i2 / 4] - mo[t2]));
+                } else {
+                    const float by[2] = {__builtin_amdgcn_exp2f(r0), __builtin_amdgcn_exp2f(r1)};
+#pragma unroll
+                    for (int i2 = 0; i2 < 8; ++i2) y[i2] *= by[i2 / 4];
+                }
 #pragma unroll
                 for (int i2 = 0; i2 < 8; i2 += 2) {
                     const f16x2 w = __builtin_convertvector((f32x2{y[i2], y[i2 + 1]}), f16x2);
@@ -346,21 +345,31 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
         if (g == 0) {
             stat[0][wave][t * 16 + n16] = m[t];
             stat[1][wave][t * 16 + n16] = l[t];
+            stat[2][wave][t * 16 + n16] = mo[t];
         }
     }
     __syncthreads();
     float total[NT], high[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+        float high_o = kNone;
         high[t] = kNone;
         total[t] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) high[t] = fmaxf(high[t], stat[0][w][t * 16 + n16]);
+        for (int w = 0; w < kWaves; ++w) {
+            high[t] = fmaxf(high[t], stat[0][w][t * 16 + n16]);
+            high_o = fmaxf(high_o, stat[2][w][t * 16 + n16]);
+        }
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) total[t] += stat[1][w][t * 16 + n16] * __builtin_amdgcn_exp2f(stat[0][w][t * 16 + n16] - high[t]);
-        const float by = v_top * __builtin_amdgcn_exp2f(m[t] - high[t]);
+        const WayBack back(total[t], high_o - high[t]);
+        const float by = back.first * __builtin_amdgcn_exp2f(mo[t] - high_o);
 #pragma unroll
         for (int j = 0; j < VB; ++j) o[t][j] *= by;
+        if (back.two) {
+#pragma unroll
+            for (int j = 0; j < VB; ++j) o[t][j] *= back.second;
+        }
     }
     if (wave >= 2) {
 #pragma unroll
@@ -408,7 +417,6 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
                 }
             }
         } else {
-            const float by = total[t] > 0.0f ? 1.0f / total[t] : 0.0f;
             const uint32_t token = fast_quotient(r, a.by_group);
             uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + static_cast<int64_t>(head * a.group + (r - token * a.group)) * a.out_head;
 #pragma unroll
@@ -417,8 +425,7 @@ __global__ __launch_bounds__(kWaves *kWave, DP > 192 ? 1 : DP > 128 ? 2 : (DP <=
                 if (d >= a.dim) continue;
 #pragma unroll
                 for (int j = 0; j < VB; j += 4) {
-                    *reinterpret_cast<u32x2_any *>(p + d + j) = u32x2{narrow2_rne(a.bf16, o[t][j][i] * by, o[t][j + 1][i] * by),
-                                                                      narrow2_rne(a.bf16, o[t][j + 2][i] * by, o[t][j + 3][i] * by)};
+                    *reinterpret_cast<u32x2_any *>(p + d + j) = u32x2{narrow2_rne(a.bf16, o[t][j][i], o[t][j + 1][i]), narrow2_rne(a.bf16, o[t][j + 2][i], o[t][j + 3][i])};
                 }
             }
         }
@@ -432,7 +439,7 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_join(AttentionA
     constexpr int PER = DP / 64;
     __shared__ uint64_t slots[kWaves];
     __shared__ Unit shared_unit;
-    __shared__ float meet[kWaves][PER + 1][kWave];
+    __shared__ float meet[kWaves][PER][kWave];
     Unit u;
     const uint32_t head = blockIdx.x % a.kv_heads;
     if (!find_unit<kWaves, true>(a, blockIdx.x / a.kv_heads, slots, &shared_unit, &u)) return;
@@ -444,18 +451,17 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_join(AttentionA
     const uint32_t first = four ? blockIdx.y : blockIdx.y * kWaves + wave, step = four ? gridDim.y : gridDim.y * kWaves;
     for (uint32_t in_tile = first; in_tile < rows; in_tile += step) {
         const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * a.tile_rows + in_tile; };
-        float high = kNone;
-        for (uint32_t c = lane; c < u.chunks; c += kWave) high = fmaxf(high, a.part_stat[2 * at(c)]);
-        high = wave_max(high);
-        float total = 0.0f, o[PER] = {};
+        // a lane's unit of those that the wavefront adds up, and the weight of all
+        const auto unit_weight = [&](uint32_t c) { return c < c1 ? Weight{a.part_stat[2 * at(c)], a.part_stat[2 * at(c) + 1]} : Weight{kNone, 0.0f}; };
+        Weight mine = unit_weight(c0 + lane), all{kNone, 0.0f};
+        for (uint32_t c = lane; c < u.chunks; c += kWave) all.add(a.part_stat[2 * at(c)], a.part_stat[2 * at(c) + 1]);
+        const float high = wave_max(all.m);
+        all = Weight{high, wave_sum(all.l * __builtin_amdgcn_exp2f(all.m - high))};
+        const float each = all.inverse();
+        float o[PER] = {};
         for (uint32_t base = c0; base < c1; base += kWave) {
-            const uint32_t mine = base + lane;
-            float by = 0.0f, l = 0.0f;
-            if (mine < c1) {
-                l = a.part_stat[2 * at(mine) + 1];
-                by = l > 0.0f ? __builtin_amdgcn_exp2f(a.part_stat[2 * at(mine)] - high) : 0.0f;
-            }
-            total += wave_sum(l * by);
+            if (base != c0) mine = unit_weight(base + lane);
+            const float by = mine.l * __builtin_amdgcn_exp2f(mine.m - high) * each;// the part of all weights
             const uint32_t n = c1 - base < kWave ? c1 - base : kWave;
             // 16 loads under way at a time; a unit that saw nothing has written nothing, and what is read of it is not used
             for (uint32_t k0 = 0; k0 < n; k0 += 16) {
@@ -475,28 +481,24 @@ __global__ __launch_bounds__(kWaves *kWave) void paged_attention_join(AttentionA
             }
         }
         if (four) {
-            meet[wave][PER][lane] = total;
 #pragma unroll
             for (int i = 0; i < PER; ++i) meet[wave][i][lane] = o[i];
             __syncthreads();
-            total = 0.0f;
 #pragma unroll
             for (int i = 0; i < PER; ++i) o[i] = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
-                total += meet[w][PER][lane];
 #pragma unroll
                 for (int i = 0; i < PER; ++i) o[i] += meet[w][i][lane];
             }
             __syncthreads();
             if (wave != 0) continue;
         }
-        const float by = total > 0.0f ? 1.0f / total : 0.0f;
         const uint32_t r = row0 + in_tile, token = fast_quotient(r, a.by_group);
         uint16_t *p = a.out + static_cast<int64_t>(u.first + token) * a.out_token + static_cast<int64_t>(head * a.group + (r - token * a.group)) * a.out_head;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            if (lane * PER + i < a.dim) p[lane * PER + i] = static_cast<uint16_t>(narrow2_rne(a.bf16, o[i] * by, 0.0f));
+            if (lane * PER + i < a.dim) p[lane * PER + i] = static_cast<uint16_t>(narrow2_rne(a.bf16, o[i], 0.0f));
         }
     }
 }

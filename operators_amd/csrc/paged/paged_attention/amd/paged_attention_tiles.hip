@@ -10,8 +10,12 @@
 // the next is written and the one behind it is on its way from memory.
 // v_mfma_f32_32x32x16 leaves a lane 16 of the 32 keys of one query, and V's keys lie in
 // the order in which those make up the second product's operand, so P is not exchanged.
-// The V scale of a block is added to the exponent (P = exp2(x - m + log2 r)) and taken
-// out of its sum again (sum / r), which saves a product for each score.
+// The V scale of a block, r times the largest so far, is added to the exponent, and taken out
+// of its sum again, which saves a product for each score:
+//     P = exp2(score + log2 r - m),  l = sum(P / r),  out = V^T P (largest V scale) / l
+// m is the running maximum of score + log2 r less 10, each query row's own, so that what fp16
+// holds of P depends only on what the row sees and gives weight to.  "The largest" is of the keys that
+// some of the wavefront's 32 rows see; it keeps l in range, and a scale below 2^-80 of it counts as that.
 // Two wavefronts share a SIMD and are a phase apart: one at its products, the other at
 // its exponentials and the next tile's codes (when that took 330 us in the example
 // below: 353 without, 390 with wavefronts of the same phase on a SIMD).
@@ -30,7 +34,8 @@ namespace {
 using namespace amd;
 
 constexpr float kLift = 10.0f, kSlack = 4.0f, kNone = -1.0e30f;// as in paged_attention_rows.hip
-constexpr float kLeastRatio = -40.0f;// log2 of a V scale to the largest: P times it is 0 in fp16
+constexpr float kLeastRatio = -80.0f;// log2 of a V scale to the largest: l stays below 2^(14 + 80 + 31)
+constexpr float kZeroScale = -1000.0f;// log2 of a V scale of 0, and of one that nobody sees
 
 __device__ __forceinline__ float pair_max(float v) {
     return across32(v, [](float a, float b) { return fmaxf(a, b); });
@@ -311,25 +316,29 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
     }
-    // the running maximum less 10, its sum, and log2 of the largest V scale so far, which O stands relative to
+    // the running maximum less 10 of score + v_rel, which l is relative to, and log2 of the largest V scale so far, which O is too
     float m = kNone, l = 0.0f, v_top = kNone;
     float k_scale, v_rel, v_back;// of the lane's group: of V log2 relative to v_top, and the way back
     uint64_t no_page = 0;        // a bit for each group
     const auto scales = [&](uint32_t tile) {
         const int page = page_of(tile);
-        float v_log = -200.0f;
+        float v_log = kZeroScale;
         k_scale = 0.0f;
         if (page >= 0) {
-            const uint32_t block = fast_quotient(place_of(first_key + tile * BK + seldom(lane) * 16), a.by_block);
+            const uint32_t key = first_key + tile * BK + seldom(lane) * 16, block = fast_quotient(place_of(key), a.by_block);
             k_scale = ks_base[page * a.k_at.s_page + block];
-            v_log = __builtin_amdgcn_logf(fmaxf(vs_base[page * a.v_at.s_page + block], 0x1p-126f));
+            if (key < some_see) v_log = fmaxf(log2_of(vs_base[page * a.v_at.s_page + block]), kZeroScale);
         }
         asm volatile("" : "+v"(k_scale));// (waited for here, not where this way and the one past it meet)
         no_page = __builtin_amdgcn_ballot_w64(page < 0);
         const float v_now = wave_max(v_log);
         if (v_now > v_top) {
-            const float by = __builtin_amdgcn_exp2f(v_top - v_now);
+            // all v_rel so far fall by `up`, and m with them, as far as l stays below 2^90; what O is beyond that goes into O
+            const float up = v_now - v_top, down = fminf(up, fminf(120.0f, 90.0f - __builtin_amdgcn_logf(pair_max(l))));
+            const float by = __builtin_amdgcn_exp2f(down - up);
             v_top = v_now;
+            m -= down;
+            l *= __builtin_amdgcn_exp2f(down);
 #pragma unroll
             for (int t = 0; t < TD; ++t) o[t] *= by;
         }
@@ -339,7 +348,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
 
     // The scores of a tile as the matrix units leave them, and what they are multiplied by.
     f32x16 s[NB];
-    float f[NG], high = kNone;
+    float f[NG], rel[NG], high = kNone;
     const auto products = [&](uint32_t tile) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -355,7 +364,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             }
         }
     };
-    // The largest score, from the largest product of each group.
+    // The largest score + v_rel, from the largest product of each group.
     const auto largest = [&](uint32_t tile) {
         const uint32_t at = tile % kAhead * NG;
         high = kNone;
@@ -366,7 +375,8 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             const f32x16 &x = s[g / 2];
             const int b = g % 2 * 8;
             const float top = fmaxf(fmaxf(fmaxf(fmaxf(x[b], x[b + 1]), x[b + 2]), fmaxf(fmaxf(x[b + 3], x[b + 4]), x[b + 5])), fmaxf(x[b + 6], x[b + 7]));
-            high = fmaxf(high, top * f[g]);
+            rel[g] = lane_of(v_rel, at + g);
+            high = fmaxf(high, __builtin_fmaf(top, f[g], rel[g]));
         }
     };
     // What a tile's scores need before their exponentials: the mask and the maximum.
@@ -430,7 +440,7 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
             const uint32_t now = tile % kAhead * NG;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float less = lane_of(v_rel, now + g) - m;
+                const float less = rel[g] - m;
                 float y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + i], f[g], less));
@@ -484,7 +494,13 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
 
     if (!any) return;
     l = across32(l, [](float x, float y) { return x + y; });
-    const float v_unit = __builtin_amdgcn_exp2f(fmaxf(v_top, -140.0f));
+    const WayBack back(l, v_top);
+#pragma unroll
+    for (int t = 0; t < TD; ++t) o[t] *= back.first;
+    if (back.two) {
+#pragma unroll
+        for (int t = 0; t < TD; ++t) o[t] *= back.second;
+    }
     if (u.chunks > 1) {// as the lanes hold it, 16 bytes of each side by side
         const uint64_t at = (static_cast<uint64_t>(u.slot + u.chunk) * a.kv_heads + head) * kWaves + wave;
         if (h == 0) {
@@ -494,13 +510,12 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         float *p = a.part_out + at * (32 * DP) + lane * 4;
 #pragma unroll
         for (int k = 0; k < 16 * TD; k += 4) {
-            const auto of = [&](int j) { return o[(k + j) % TD][(k + j) / TD] * v_unit; };
+            const auto of = [&](int j) { return o[(k + j) % TD][(k + j) / TD]; };
             *reinterpret_cast<f32x4 *>(p + k * kWave) = f32x4{of(0), of(1), of(2), of(3)};
         }
     } else {
-        const float by = l > 0.0f ? v_unit / l : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) put_four<DP>(a, n32, h, scratch, i / 4, [&](int t, int j) { return o[t][i + j] * by; });
+        for (int i = 0; i < 16; i += 4) put_four<DP>(a, n32, h, scratch, i / 4, [&](int t, int j) { return o[t][i + j]; });
         put_rows<DP>(a, my_rows, lane, scratch);
     }
 }
@@ -520,18 +535,18 @@ __global__ __launch_bounds__(4 * kWave) void paged_attention_tiles_join(Attentio
     const uint32_t tokens = u.count < a.max_tokens ? u.count : a.max_tokens, rows = tokens * a.group, mine0 = u.tile * a.tile_rows + part * 32;
     if (mine0 >= rows) return;
     const auto at = [&](uint32_t c) { return (static_cast<uint64_t>(u.slot + c) * a.kv_heads + head) * waves + part; };
-    float high = kNone;
+    const auto stat = [&](uint32_t c, int i) { return a.part_stat[2 * (at(c) * 32 + n32) + i]; };
+    Weight all{kNone, 0.0f};
 #pragma unroll 4
-    for (uint32_t c = 0; c < u.chunks; ++c) high = fmaxf(high, a.part_stat[2 * (at(c) * 32 + n32)]);
+    for (uint32_t c = 0; c < u.chunks; ++c) all.add(stat(c, 0), stat(c, 1));
+    const float each = all.inverse();
     f32x4 o[TD];
 #pragma unroll
     for (int t = 0; t < TD; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float total = 0.0f;
 #pragma unroll 4
     for (uint32_t c = 0; c < u.chunks; ++c) {
         const float *p = a.part_out + at(c) * (32 * DP) + wave * (4 * TD * kWave) + lane * 4;
-        const float l = a.part_stat[2 * (at(c) * 32 + n32) + 1], by = __builtin_amdgcn_exp2f(a.part_stat[2 * (at(c) * 32 + n32)] - high);
-        total += l * by;
+        const float by = stat(c, 1) * __builtin_amdgcn_exp2f(stat(c, 0) - all.m) * each;// its part of all weights
 #pragma unroll
         for (int k = 0; k < TD; ++k) {
             const f32x4 x = ld16f(p + k * 4 * kWave);
@@ -539,8 +554,7 @@ __global__ __launch_bounds__(4 * kWave) void paged_attention_tiles_join(Attentio
             for (int j = 0; j < 4; ++j) o[(k * 4 + j) % TD][(k * 4 + j) / TD] += x[j] * by;
         }
     }
-    const float by = total > 0.0f ? 1.0f / total : 0.0f;
-    put_four<DP>(a, n32, lane >> 5, scratch, wave, [&](int t, int j) { return o[t][j] * by; });
+    put_four<DP>(a, n32, lane >> 5, scratch, wave, [&](int t, int j) { return o[t][j]; });
     __syncthreads();
     put_rows<DP, 4 * kWave>(a, TileRows{mine0, rows - mine0 < 32 ? rows - mine0 : 32, u.first, head}, tid, scratch);
 }

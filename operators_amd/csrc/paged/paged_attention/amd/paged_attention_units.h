@@ -29,7 +29,7 @@ struct AttentionArgs {
     uint32_t whole_steps;
     uint32_t least_rows, most_rows;// of a sequence that this kernel takes
     bool bf16;
-    float *part_out, *part_stat;// [slot, kv head][tile row][padded dim], and [..][2]
+    float *part_out, *part_stat;// [slot, kv head][tile row][padded dim]: a unit's own result, and [..][2]: m and l, its weight
 };
 
 struct Unit {
@@ -177,6 +177,33 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, uint32_t index
                 same(shared->count), same(shared->length), same(shared->steps), same(shared->slot)};
     return true;
 }
+
+// log2, of subnormal numbers too, which the instruction takes as 0; minus infinity of 0.
+__device__ __forceinline__ float log2_of(float v) {
+    const bool low = v < 0x1p-100f;
+    return __builtin_amdgcn_logf(low ? v * 0x1p100f : v) - (low ? 100.0f : 0.0f);
+}
+// A unit's weight beside others': l relative to 2^m, several of them together.
+struct Weight {
+    float m, l;
+    __device__ __forceinline__ void add(float m2, float l2) {
+        const float next = fmaxf(m, m2);
+        l = l * __builtin_amdgcn_exp2f(m - next) + l2 * __builtin_amdgcn_exp2f(m2 - next);
+        m = next;
+    }
+    __device__ __forceinline__ float inverse() const { return l > 0.0f ? 1.0f / l : 0.0f; }// 0 where nothing was seen
+};
+// What O is multiplied by, 2^exponent / l, as one factor or, where that may be out of range (V scales reach from 2^-149 to
+// 2^127), as two.
+struct WayBack {
+    float first, second;
+    bool two;// the same for the whole wavefront
+    __device__ __forceinline__ WayBack(float l, float exponent) {
+        two = __builtin_amdgcn_ballot_w64(fabsf(exponent) > 60.0f || l > 0x1p50f) != 0;
+        second = two ? __builtin_amdgcn_exp2f(0.5f * exponent) : 1.0f;
+        first = Weight{0.0f, l}.inverse() * (two ? second : __builtin_amdgcn_exp2f(exponent));
+    }
+};
 
 // 16-bit results, to nearest even
 __device__ __forceinline__ uint32_t narrow2_rne(bool bf16, float a, float b) {

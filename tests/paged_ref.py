@@ -124,6 +124,26 @@ def attention_bound(want, mean, size, dtype, dim, length, v_top):
     return inside + eps * (want.abs() + inside) + tiny
 
 
+def largest_share(q, k, v_scale, cache, scale, there=None):
+    """[tokens, heads]: the largest that one key which the token sees could add to its result, weight times V scale times the largest code.
+    v_scale: [length, kv_heads]."""
+    tokens, heads, _ = q.shape
+    length, kv, _ = k.shape
+    there = torch.ones(length, dtype=torch.bool) if there is None else there
+    kk = torch.where(there[:, None, None], k, 0.0).repeat_interleave(heads // kv, 1)
+    s = torch.einsum("thd,jhd->thj", q.double(), kk) * scale
+    seen = (torch.arange(length)[None, :] <= (length - tokens + torch.arange(tokens))[:, None]) & there[None, :]
+    p = torch.softmax(s.masked_fill(~seen[:, None], -float("inf")), -1)
+    one = torch.where(there[:, None], v_scale.double(), 0.0).repeat_interleave(heads // kv, 1)
+    return torch.where(p.isnan(), 0.0, p * one.T[None]).amax(-1) * MOST[cache]
+
+
+def seen_bound(want, mean, size, dtype, dim, length, share):
+    """attention_bound with its point on small weights held to what each token sees: a weight times its V scale that is too small
+    for fp16 is off by 2^-35 of the largest such product (`share`, of the token itself), times the largest code, for each key."""
+    return attention_bound(want, mean, size, dtype, dim, length, share[..., None])
+
+
 # ---- page tables ----------------------------------------------------------------
 def update(table, lengths, refs, source, grow, page):
     """(table, lengths, refs, pairs, result) after PageTableUpdate, from lists."""

@@ -310,6 +310,111 @@ def test_prompts_past_missing_pages(ctx, dim, cache):
         p.check(p.run(ctx))
 
 
+class Seen(Problem):
+    """A problem whose V scales are changed by `change(scales of v, pages of the rows)`, held to a bound that takes of each token's
+    keys only those that it sees, by the weights that they have."""
+
+    def __init__(self, rows, change, **more):
+        super().__init__(rows, garbage=False, **more)
+        side, (_, gpu) = self.sides[1], self.gpu[1]
+        change(side.scales, self.table)
+        gpu.copy_(side.scales)
+
+    def check(self, out, least=0.0):
+        """least: a V scale smaller than this part of the largest may count as that.  What this adds is rounded with the rest: to bf16
+        (2^-8 of it), its weight to fp16 (2^-11) and by its scale's exponent (2^-16), less than 2^-7 of it together."""
+        out = out.cpu()
+        assert torch.isfinite(out.float()).all()
+        for r, (had, new) in enumerate(self.rows):
+            lo, n = int(self.offsets[r]), had + new
+            if not new:
+                continue
+            pages = self.table[r].tolist()
+            k, v = (s.read(pages, n) for s in self.sides)
+            want, mean, size = ref.attention(self.q[lo:lo + new], k, v, self.scale)
+            side = self.sides[1]
+            scales = torch.stack([side.scales[pages[j // side.page], :, j % side.page // side.block] for j in range(n)])
+            share = ref.largest_share(self.q[lo:lo + new], k, scales, self.cache, self.scale)
+            bound = ref.seen_bound(want, mean, size, self.dtype, self.dim, n, share) + least * float(scales.max()) * ref.MOST[self.cache] * (1 + 2.0 ** -7)
+            off = (out[lo:lo + new].double() - want).abs()
+            assert (off <= bound).all(), (r, had, new, float((off / bound).max()), int((off > bound).any(-1).any(-1).nonzero()[0]))
+
+
+def times(exponent, start, end=None):
+    """The V scales of blocks start .. end of every row, by a power of two."""
+    def change(scales, table):
+        per = scales.shape[2]
+        for row in table.tolist():
+            held = [(p, b) for p in row if p >= 0 for b in range(per)]
+            for p, b in held[start:end]:
+                scales[p, :, b] *= 2.0 ** exponent
+    return change
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("exponent, dim", [(-26, 64), (-34, 64), (-60, 64), (-34, 256), (-60, 256)])
+@pytest.mark.parametrize("rows, heads, kv_heads", [([(14, 5), (30, 2)], 4, 2), ([(0, 12), (14, 4)], 16, 2), ([(14, 150), (0, 300)], 8, 2), ([(15, 70)], 1, 1),
+                                                   ([(14, 40)], 8, 2), ([(0, 1100)], 4, 2)], ids=str)
+def test_values_far_smaller_than_the_unseen(ctx, rows, heads, kv_heads, exponent, dim, cache):
+    """The first block's values are smaller than all later ones by far, which the first tokens do not see."""
+    p = Seen(rows, times(exponent, 0, 1), heads=heads, kv_heads=kv_heads, dim=dim, cache=cache, dtype="bf16", seed=heads)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("new", [1, 20, 100])
+@pytest.mark.parametrize("exponent", [30, 60])
+@pytest.mark.parametrize("k_scale", [1.0, 2.0 ** -6])
+def test_values_far_smaller_than_the_unweighted(ctx, k_scale, exponent, new):
+    """A block of huge values whose weight is next to nothing, before, between and behind the others."""
+    for block in (0, 7, 20):
+        p = Seen([(340, new)], times(exponent, block, block + 1), heads=8, kv_heads=2, dim=64, cache="e4m3", dtype="bf16", seed=block)
+        k, (codes, _) = p.sides[0], p.gpu[0]
+        page, at = int(p.table[0, block // 2]), block % 2 * 16
+        low = torch.full((16,), -240.0).to(torch.float8_e4m3fn).view(torch.uint8)[0]
+        k.codes.view(torch.uint8)[page, :, at:at + 16] = low  # all products far below 0
+        k.scales[page, :, block % 2] = k_scale
+        codes.view(torch.uint8).copy_(k.codes.view(torch.uint8))
+        p.gpu[0][1].copy_(k.scales)
+        p.q = p.q.abs()
+        p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("rows", [[(3100, 1), (2050, 3)], [(2900, 200)], [(1000, 60), (2100, 40), (3000, 33)], [(0, 1100)]], ids=str)
+@pytest.mark.parametrize("steps", [(-120, -60, 0), (0, -60, -120), (-90, 0, -90), (-40, -39, 0)])
+@pytest.mark.parametrize("q_scale", [0.0, 1.0, 40.0])
+def test_values_that_jump_along_the_row(ctx, q_scale, steps, rows):
+    """V scales that rise and fall by up to 2^120 every 1024 keys, with weights from equal ones to nearly one."""
+    def change(scales, table):
+        for i, e in enumerate(steps):
+            times(e, i * 64, None if i == 2 else i * 64 + 64)(scales, table)
+    p = Seen(rows, change, heads=2, kv_heads=1, dim=64, cache="e4m3", dtype="bf16", seed=11, q_scale=q_scale)
+    p.check(p.run(ctx), least=2.0 ** -80)
+
+
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("exponent", [-135, -100, 100, 118])
+@pytest.mark.parametrize("rows", [[(40, 1), (0, 3)], [(9000, 1)], [(300, 90)], [(5000, 60), (3, 1)]], ids=str)
+def test_values_near_the_ends_of_the_type(ctx, rows, exponent, cache):
+    """V scales from subnormal numbers up to values of 2^120: results of 16 bits hold them, and so does all on the way."""
+    p = Seen(rows, times(exponent, 0), heads=8, kv_heads=1, dim=128, cache=cache, dtype="bf16", seed=5)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("new", [1, 50])
+def test_scales_of_zero(ctx, new):
+    """A V scale of 0 stands for zeros whatever the codes, all along a row and in its first and last blocks; the weights count."""
+    for start, end in ((0, None), (0, 20), (30, None)):
+        def change(scales, table):
+            pages = [p for p in table[0].tolist() if p >= 0]
+            for i in range(start, len(pages) * 2 if end is None else end):
+                scales[pages[i // 2], :, i % 2] = 0
+        p = Seen([(900, new)], change, heads=8, kv_heads=2, dim=64, cache="i8", dtype="bf16", seed=2)
+        out = p.run(ctx)
+        p.check(out)
+        if start == 0 and end is None:
+            assert (out[:new] == 0).all()
+
+
 # ---- more than 64 rows: the units are found by a scan over the workgroup ------------
 @pytest.mark.parametrize("cache", ["i8", "e4m3"])
 @pytest.mark.parametrize("count", [65, 257, 300])
