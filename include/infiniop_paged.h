@@ -52,8 +52,8 @@ static const DataLayout F8E4M3 = INFINIOP_DT(1, 1, 1, 3, 4);
  * and, where the block holds older tokens of the row, at least the scale that
  * it has; their codes are brought to a scale that grew,
  *     code = round(code * (old scale / scale)).
- * New values become round(x * (1 / scale)), in fp32, to nearest even, infinities
- * the largest code of their sign, NaN 0 (and 0 where the scale is 0).  The places
+ * New values become round(x * (1 / scale)), in fp32, to nearest even, what is
+ * beyond the codes (infinities too) the largest of its sign, NaN 0 (and 0 where the scale is 0).  The places
  * behind a row's last token keep what they hold.  Two rows that call may not store
  * into one page (a page that rows share is copied on write by PageTableUpdate).
  * ======================================================================== */

@@ -85,7 +85,7 @@ __device__ __forceinline__ u16x2 top_finite(const u32x4 (&w)[2], u16x2 top) {
     return top;
 }
 
-// 16 values times inv, to the nearest code.  ANY: also infinities (to the ends) and NaN (to 0); else the products are
+// 16 values times inv, to the nearest code.  ANY: also beyond the codes (to the ends) and NaN (to 0); else the products are
 // within the codes, for the scale is at least the top's.
 template<bool FP8, bool ANY>
 __device__ __forceinline__ u32x4 codes_of(const float (&x)[16], float inv) {
@@ -270,7 +270,8 @@ __global__ __launch_bounds__(kAppendWaves *kWave) void kv_cache_append(AppendArg
         float x[16];
         widen16<T>(w, x);
         u32x4 c;
-        if (any || now == 0.0f) c = codes_of<FP8, true>(x, inv);
+        // (a scale below 2^-96 is 0, or an older one that values which count as 0 may exceed, or whose inverse is infinite)
+        if (any || now < 0x1p-96f) c = codes_of<FP8, true>(x, inv);
         else c = codes_of<FP8, false>(x, inv);
         *reinterpret_cast<u32x4 *>(codes + static_cast<uint64_t>(lo + token) * at.token + (e - token * per_token) * 16) = c;
     };

@@ -248,6 +248,27 @@ def test_append_more_than_1024_rows(ctx):
     check_append(ctx, [((3 * r) % 20, 0 if r % 2 else 2) for r in range(1100)], cache="i8", dim=16, heads=1, page=16, dtype="bf16")
 
 
+@pytest.mark.parametrize("page, block, dim", [(32, 32, 64), (256, 256, 64)])
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("scale", [1e-45, 1e-40, 2.0 ** -127, 2.0 ** -110])
+def test_append_onto_scales_of_next_to_nothing(ctx, scale, cache, page, block, dim):
+    """Older tokens whose scale has no finite inverse, or is smaller than new values that count as 0: zeros stay zeros and what
+    is beyond the codes becomes the largest."""
+    for value in (0.0, 2.0 ** -97, 1e-38, float("inf"), float("nan")):
+        codes, scales = make_cache(2, 2, page, dim, block, cache, 3)
+        scales.fill_(scale)
+        x = torch.zeros(3, 2, dim, dtype=torch.bfloat16)
+        x[1, 0, ::2], x[1, 0, 1::4], x[2, 1, 5] = value, -value, value
+        sides = [ref.Cache(codes.clone(), scales.clone(), cache) for _ in range(2)]
+        kc, vc, ks, vs = codes.to(DEV), codes.to(DEV), scales.to(DEV), scales.to(DEV)
+        ctx.kv_cache_append(kc, vc, ks, vs, x.to(DEV), -x.to(DEV), torch.tensor([[1]], dtype=torch.int32, device=DEV),
+                            torch.tensor([0, 3], dtype=torch.int32, device=DEV), torch.tensor([8], dtype=torch.int32, device=DEV))
+        torch.cuda.synchronize()
+        for side, new, c, s in zip(sides, (x, -x), (kc, vc), (ks, vs)):
+            side.append([1], 5, new)
+            assert same(s, side.scales) and same(c, side.codes), value
+
+
 # ---- KVCacheCopy ---------------------------------------------------------------
 @pytest.mark.parametrize("layout", ["dense", "tokens first", "wide"])
 @pytest.mark.parametrize("dim, heads, page, block, pages", [(16, 1, 16, 16, 5), (80, 3, 48, 16, 9), (128, 8, 64, 32, 20), (256, 2, 128, 128, 6)])
