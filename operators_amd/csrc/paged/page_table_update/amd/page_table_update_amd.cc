@@ -28,7 +28,7 @@ infiniopStatus_t amdCreatePageTableUpdateDescriptor(AmdHandle_t handle, PageTabl
     // the bits of the free pages and their count by chunk; a row's length before it grows and its growth; the rows that change
     const uint64_t chunks = amd::chunks_of(sizes.pages);
     const uint64_t bytes = chunks * kChunkWords * 8 + chunks * 4 + rows * 8 + rows * sizes.old_rows.cols * 4;
-    auto *desc = new (std::nothrow) PageTableUpdateAmdDescriptor{DevAmdGpu, handle->device_id, sizes, rows == 0 ? 0 : bytes};
+    auto *desc = new (std::nothrow) PageTableUpdateAmdDescriptor{DevAmdGpu, handle->device_id, sizes, bytes};
     if (desc == nullptr) {
         return STATUS_MEMORY_NOT_ALLOCATED;
     }

@@ -323,15 +323,16 @@ infiniopStatus_t amdPageTableUpdate(PageTableUpdateAmdDescriptor_t desc, void *w
                                     void const *source, void const *grow, void *stream) {
     const PageTableUpdateAmdDescriptor &d = *desc;
     const amd::TableSizes &z = d.sizes;
-    if (z.old_rows.rows == 0) {
-        return STATUS_SUCCESS;
-    }
     if (workspace == nullptr || workspace_size < d.workspace) {
         return STATUS_MEMORY_NOT_ALLOCATED;
     }
-    for (const void *p : {static_cast<const void *>(new_table), static_cast<const void *>(new_lengths), static_cast<const void *>(new_refcount),
-                          static_cast<const void *>(pairs), static_cast<const void *>(result), table, lengths, refcount, source, grow}) {
+    for (const void *p : {static_cast<const void *>(new_refcount), static_cast<const void *>(result), refcount}) {
         if (p == nullptr) return STATUS_BAD_PARAM;
+    }
+    // (no rows: the counts and the result are written all the same)
+    for (const void *p : {static_cast<const void *>(new_table), static_cast<const void *>(new_lengths), static_cast<const void *>(pairs), table, lengths,
+                          source, grow}) {
+        if (p == nullptr && z.old_rows.rows != 0) return STATUS_BAD_PARAM;
     }
     if (reinterpret_cast<uintptr_t>(workspace) % 8 != 0 || (new_table == table && z.new_rows.stride != z.old_rows.stride)) {
         return STATUS_BAD_PARAM;
@@ -353,7 +354,7 @@ infiniopStatus_t amdPageTableUpdate(PageTableUpdateAmdDescriptor_t desc, void *w
         if (most <= 4 * kSmallLanes) page_table_update_small<4><<<1, kSmallLanes, 0, s>>>(a, by_cols);
         else page_table_update_small<kSmallEach><<<1, kSmallLanes, 0, s>>>(a, by_cols);
     } else {
-        const unsigned by_row = static_cast<unsigned>(rows < 1024 ? rows : 1024), by_chunk = static_cast<unsigned>(chunks < 1024 ? chunks : 1024);
+        const unsigned by_row = static_cast<unsigned>(rows == 0 ? 1 : rows < 1024 ? rows : 1024), by_chunk = static_cast<unsigned>(chunks < 1024 ? chunks : 1024);
         page_table_rows<<<by_row, kTableWaves * amd::kWave, 0, s>>>(a);
         page_table_count<<<by_row, kTableWaves * amd::kWave, 0, s>>>(a);
         page_table_needs<<<by_row > by_chunk ? by_row : by_chunk, kTableWaves * amd::kWave, 0, s>>>(a);

@@ -108,6 +108,17 @@ def test_update_edges(ctx, large):
     assert check([3, 1, 2, 3, 4, 5], [1, 0, 0, 1, 0, 0], lengths=[20, 33, 16, 20, 48, 0]) == [0, 0]
 
 
+@pytest.mark.parametrize("pages", [5, 30000])
+def test_update_of_no_rows(ctx, pages):
+    """A batch without rows: the counts stay, and nothing lacks."""
+    none, refs = torch.zeros(0, dtype=torch.int32, device=DEV), ints([p % 3 for p in range(pages)])
+    table, pairs = torch.zeros(0, 4, dtype=torch.int32, device=DEV), torch.zeros(0, 2, dtype=torch.int32, device=DEV)
+    for out in (torch.full_like(refs, 99), refs):
+        result = ints([99, 99])
+        ctx.page_table_update(table, none, out, pairs, result, table, none, refs, none, none, 16)
+        assert result.tolist() == [0, 0] and out.tolist() == [p % 3 for p in range(pages)]
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("rows, cols, pages, page, most", SIZES)
 def test_compact(ctx, rows, cols, pages, page, most, in_place):
