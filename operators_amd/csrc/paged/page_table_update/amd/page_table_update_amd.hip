@@ -17,8 +17,9 @@ namespace {
 using namespace amd;
 
 constexpr int kTableWaves = 4;
-// a row's growth: its pages, and whether the first of them takes the place of the last page
-constexpr uint32_t kCopies = 1u << 31, kTooWide = 1u << 30;
+// a row's growth: its pages (below 2^31; only pages of several tokens are copied, and then it is below 2^30), and whether
+// the first of them takes the place of the last page
+constexpr uint32_t kCopies = 1u << 31, kTooWide = ~0u;
 
 struct UpdateArgs {
     const int *table, *lengths, *refcount, *source, *grow;

@@ -119,6 +119,17 @@ def test_update_of_no_rows(ctx, pages):
         assert result.tolist() == [0, 0] and out.tolist() == [p % 3 for p in range(pages)]
 
 
+def test_update_that_wants_2_30_pages(ctx):
+    """Pages of one token and a row that grows by 2^30 of them: it is not too wide, the pages lack."""
+    cols = (1 << 30) + 3
+    table = torch.full((1, cols), -1, dtype=torch.int32, device=DEV)
+    refs, length, result, pairs = ints([0] * 100), ints([0]), ints([9, 9]), ints([[9, 9]])
+    for grow, want in (((1 << 30) - 1, [(1 << 30) - 101, 0]), (1 << 30, [(1 << 30) - 100, 0]), ((1 << 30) + 1, [(1 << 30) - 99, 0]), ((1 << 30) + 4, [0, 1])):
+        ctx.page_table_update(table, length, refs, pairs, result, table, length, refs, ints([0]), ints([grow]), 1)
+        assert result.tolist() == want, grow
+        assert length.tolist() == [0] and pairs.tolist() == [[-1, -1]] and int(refs.sum()) == 0
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("rows, cols, pages, page, most", SIZES)
 def test_compact(ctx, rows, cols, pages, page, most, in_place):
