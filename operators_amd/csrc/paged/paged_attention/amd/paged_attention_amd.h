@@ -9,6 +9,13 @@ constexpr uint32_t paged_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 
 // Wavefronts of 32 query rows each that a workgroup of the kernel for prompts has.
 constexpr int paged_tile_waves(int padded) { return padded <= 128 ? 8 : 4; }
 
+// Steps of a unit that has at least `wanted`, at least `least`, in multiples of `whole` (a power of two).  No row has more than
+// 2^26 (places below 2^31), so that 2^30 cut nothing; more wanted ones would not fit the whole number.
+constexpr uint32_t paged_unit_steps(float wanted, uint32_t least, uint32_t whole) {
+    const uint32_t steps = wanted < 0x1p30f ? static_cast<uint32_t>(wanted) + 1 : 1u << 30;
+    return ((steps < least ? least : steps) + whole - 1) & ~(whole - 1);
+}
+
 // How a call's work is cut up.  A tile is up to `tile_rows` query rows (token by
 // head of one K/V head's group) of one sequence; a unit is a tile over a range of
 // keys, and what one workgroup computes.  `target` units of a K/V head or up to three

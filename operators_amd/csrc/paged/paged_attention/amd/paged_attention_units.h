@@ -69,9 +69,7 @@ template<typename F>
 __device__ __forceinline__ uint32_t unit_steps(const AttentionArgs &a, float total, F sum) {
     const auto cut = [&](float by) {
         // at least total / target, with room for the roundings on the way
-        uint32_t steps = static_cast<uint32_t>(total * a.units_each * by * 1.00001f) + 1;
-        steps = steps < a.least_steps ? a.least_steps : steps > 0x40000000u ? 0x40000000u : steps;
-        return (steps + a.whole_steps - 1) & ~(a.whole_steps - 1);
+        return paged_unit_steps(total * a.units_each * by * 1.00001f, a.least_steps, a.whole_steps);
     };
     if (a.rounds_each == 0.0f) return cut(1.0f);
     float least = __builtin_inff();

@@ -291,6 +291,35 @@ def test_page_table_refusals(op, args):
     assert getattr(lib, f"infiniopGet{op}WorkspaceSize")(None, None) == PARAM
 
 
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no C++ compiler")
+def test_units_of_rows_that_are_long_together(tmp_path):
+    """How long a unit of attention is, as the kernels work it out, where the rows' steps exceed 2^32 together: 64 rows of 2^31 places
+    and one unit to be made of each of 256 K/V heads.  A number that wrapped around would cut them into more units than the grid
+    and the workspace have room for."""
+    tu, exe = tmp_path / "steps.cc", tmp_path / "steps"
+    tu.write_text('''#include "paged/paged_attention/amd/paged_attention_amd.h"
+#include <cstdio>
+#include <cstdlib>
+int main(int n, char **v) {
+    for (int i = 1; i + 2 < n; i += 3) std::printf("%u\\n", paged_unit_steps(std::strtof(v[i], nullptr), std::atoi(v[i + 1]), std::atoi(v[i + 2])));
+}
+''')
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    res = subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(ROOT, "include"), "-I", os.path.join(ROOT, "operators_amd", "csrc"),
+                          "-isystem", os.path.join(rocm, "include"), str(tu), "-o", str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    wanted = [0.0, 0.5, 7.0, 15.9, 16.0, 100.5, 2.0 ** 20, 2.0 ** 26, 2.0 ** 29 + 64, 2.0 ** 30, 2.0 ** 31, 2.0 ** 32 - 256, 2.0 ** 32, 1.5 * 2.0 ** 32, 2.0 ** 40, 1e30]
+    for least, whole in ((4, 1), (8, 1), (16, 2)):
+        out = subprocess.run([str(exe)] + [str(x) for w in wanted for x in (w, least, whole)], capture_output=True, text=True, check=True).stdout.split()
+        for w, steps in zip(wanted, map(int, out)):
+            assert steps >= least and steps % whole == 0 and steps >= min(w, 2 ** 30) and steps <= max(w + 2, least, 2) and steps <= 2 ** 30, (w, steps)
+    total, longest = 64 * 2 ** 26, 2 ** 26
+    for by in (1.5, 1.25, 1.0, 2 / 3, 0.5, 1 / 3):
+        out = int(subprocess.run([str(exe), str(total * by * 1.00001), "16", "2"], capture_output=True, text=True, check=True).stdout)
+        units = 64 * -(-longest // out)
+        assert units <= 64 + total / (total * by) and (units == 64 or units <= 2 * total / (total * by)), by
+
+
 def test_no_fallback():
     with pytest.raises(FileNotFoundError):
         oa.open_paged_lib("/nonexistent/libinfiniop_paged.so")
