@@ -105,8 +105,9 @@ INFINIOP_C INFINIOP_EXPORT infiniopStatus_t infiniopCreatePagedAttentionDescript
     infiniopTensorDescriptor_t k_scale, infiniopTensorDescriptor_t v_scale,
     infiniopTensorDescriptor_t table, infiniopTensorDescriptor_t offsets, infiniopTensorDescriptor_t lengths,
     uint64_t max_tokens, float scale);
-/* room for what the workgroups that share a long row hand on: some MiB; a call with less is refused with
- * STATUS_MEMORY_NOT_ALLOCATED.  It may be shared by all calls that run one after the other. */
+/* room for what the workgroups that share a long row hand on, as far as the table is long enough for that: for decoding
+ * up to 16 to 33 MiB, for prompts up to 65 (one row) or 200 MiB, more only with more than 256 K/V heads, and 16 bytes where
+ * no row is long enough; a call with less is refused with STATUS_MEMORY_NOT_ALLOCATED.  It may be shared by all calls that run one after the other. */
 INFINIOP_C INFINIOP_EXPORT infiniopStatus_t infiniopGetPagedAttentionWorkspaceSize(infiniopPagedAttentionDescriptor_t desc, uint64_t *size);
 INFINIOP_C INFINIOP_EXPORT infiniopStatus_t infiniopPagedAttention(
     infiniopPagedAttentionDescriptor_t desc, void *workspace, uint64_t workspace_size,

@@ -9,10 +9,19 @@ namespace {
 // there and with the kernel for prompts: 64 rows of 32 x 8192 keys 195 and 246, of 8 x 800 22.6 and 29.7; 96 rows of 32 x 8192 280 and 251).
 constexpr uint32_t kFewRows = 64;
 
-// Only tiles of several units use the workspace: of those, a tile of k keys is cut at every c of them where the sum of
-// all k is at most (most_units - most_tiles) * c, so they are at most twice that many of a head (ceil(x) <= 2 x from 1 on).
+// Only tiles of several units use the workspace, and whatever offsets and lengths hold, of one head they are at most
+//   * those of tiles of k steps that are cut at every c of them, where the sum of all k is at most (most_units - most_tiles) * c:
+//     twice that many (ceil(x) <= 2 x from 1 on);
+//   * for every tile that the rows can have, the units that a row as long as the table is cut into.
+uint32_t slots_of(const PagedAttentionShape &s, const amd::PagedRows &rows, uint64_t page, uint64_t most_rows) {
+    const uint64_t by_work = 2ull * (s.most_units - s.most_tiles);
+    const uint64_t steps = amd::ceil_div(rows.cols * page, 32), units = amd::ceil_div(steps, s.least_steps);
+    if (s.most_tiles == 0 || units < 2) return 0;
+    const uint64_t tiles = rows.rows * amd::ceil_div(most_rows < s.most ? most_rows : s.most, s.tile_rows);
+    return static_cast<uint32_t>(tiles >= by_work || tiles * units >= by_work ? by_work : tiles * units);
+}
 uint64_t workspace_of(const PagedAttentionShape &s, const amd::PagedCache &c) {
-    return s.most_tiles == 0 ? 0 : 2ull * (s.most_units - s.most_tiles) * c.kv_heads * s.tile_rows * (paged_dim(c.dim) + 2) * sizeof(float);
+    return static_cast<uint64_t>(s.slots) * c.kv_heads * s.tile_rows * (paged_dim(c.dim) + 2) * sizeof(float);
 }
 
 }// namespace
@@ -74,10 +83,19 @@ infiniopStatus_t amdCreatePagedAttentionDescriptor(AmdHandle_t handle, PagedAtte
     many.target = static_cast<uint32_t>(amd::ceil_div(cus, cache.kv_heads));// one workgroup fills a compute unit
     many.at_once = rows.rows == 1 ? 0 : static_cast<uint32_t>(cus);
     many.most_units = (rows.rows == 1 ? 1 : 3) * many.target + many.most_tiles;// (one row is cut evenly)
+    // (one sequence's units begin together, and a step for each wavefront is soonest done: 300 to 4000 keys, 32/8 heads x 128,
+    // 11.2 to 12.8 us with 4, 13.1 to 14.2 with 8; where other rows' units wait, 8 of 2000 keys 20.0 with 4, 16.1 with 8)
+    few.least_steps = rows.rows == 1 ? 4 : 8;
+    few.whole_steps = 1;
+    many.least_steps = 16;
+    many.whole_steps = 2;// a tile of keys
+    few.slots = slots_of(few, rows, cache.page, most_rows);
+    many.slots = slots_of(many, rows, cache.page, most_rows);
     for (const PagedAttentionShape &s : {few, many}) {
         if (static_cast<uint64_t>(s.most_units) * cache.kv_heads > amd::max_grid_1d(512)) return STATUS_BAD_TENSOR_SHAPE;
     }
-    const uint64_t for_few = workspace_of(few, cache), for_many = workspace_of(many, cache), bytes = for_few > for_many ? for_few : for_many;
+    const uint64_t for_few = workspace_of(few, cache), for_many = workspace_of(many, cache), most = for_few > for_many ? for_few : for_many;
+    const uint64_t bytes = most > 16 ? most : 16;// (16: a call without a workspace is refused whether it needs one or not)
     auto *desc = new (std::nothrow) PagedAttentionAmdDescriptor{
         DevAmdGpu, handle->device_id, amd::same_dt(q->dt, BF16), cache, rows, static_cast<uint32_t>(tokens), static_cast<uint32_t>(group),
         static_cast<uint32_t>(max_tokens), q->strides[0], q->strides[1], out->strides[0], out->strides[1], scale, few, many,

@@ -28,6 +28,8 @@ struct PagedAttentionShape {
     uint32_t target, most_units;// most_units: of a head, whatever the lengths
     uint32_t at_once;// workgroups that the GPU holds, if units are made to fit that; 0 if not
     uint32_t least, most;
+    uint32_t least_steps, whole_steps;// of a unit: at least, and what their number is a multiple of
+    uint32_t slots;// of one K/V head: room in the workspace for the units of tiles that are cut
 };
 
 struct PagedAttentionAmdDescriptor {

@@ -513,8 +513,10 @@ void launch(const PagedAttentionAmdDescriptor &d, AttentionArgs a, hipStream_t s
         a.rounds_each = z.at_once == 0 ? 0.0f : static_cast<float>(d.cache.kv_heads) / static_cast<float>(z.at_once);
         a.least_rows = z.least;
         a.most_rows = z.most;
-        // the workspace: statistics of all slots, then their sums
-        a.part_out = a.part_stat + 4ull * (z.most_units - z.most_tiles) * d.cache.kv_heads * z.tile_rows;
+        a.least_steps = z.least_steps;
+        a.whole_steps = z.whole_steps;
+        // the workspace: weights of all slots, then their results
+        a.part_out = a.part_stat + 2ull * z.slots * d.cache.kv_heads * z.tile_rows;
         return z.most_units * d.cache.kv_heads;
     };
     // a tile of several units has two at least
@@ -524,10 +526,6 @@ void launch(const PagedAttentionAmdDescriptor &d, AttentionArgs a, hipStream_t s
     };
     if (d.few.most_tiles != 0) {
         const unsigned units = shape(d.few);
-        // (one sequence's units begin together, and a step for each wavefront is soonest done: 300 to 4000 keys, 32/8 heads x 128,
-        // 11.2 to 12.8 us with 4, 13.1 to 14.2 with 8; where other rows' units wait, 8 of 2000 keys 20.0 with 4, 16.1 with 8)
-        a.least_steps = d.rows.rows == 1 ? 4 : 8;
-        a.whole_steps = 1;
         if constexpr (DP <= 128) {
             if (d.few.tile_rows == 16) paged_attention_rows<FP8, DP, 1><<<units, kWaves * kWave, 0, s>>>(a);
             else paged_attention_rows<FP8, DP, 2><<<units, kWaves * kWave, 0, s>>>(a);
@@ -539,8 +537,6 @@ void launch(const PagedAttentionAmdDescriptor &d, AttentionArgs a, hipStream_t s
     }
     if (d.many.most_tiles != 0) {
         const unsigned units = shape(d.many);
-        a.least_steps = 16;
-        a.whole_steps = 2;
         amdLaunchPagedAttentionTiles(a, FP8, units, cut_tiles(d.many), s);
     }
 }

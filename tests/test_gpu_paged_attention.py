@@ -458,3 +458,28 @@ def test_many_rows_replayed_with_other_lengths(ctx):
             graph.replay()
             torch.cuda.synchronize()
             p.check(out)
+
+
+@pytest.mark.parametrize("rows, heads, kv_heads, dim", [([(0, 32)], 8, 1, 64), ([(511, 1)], 8, 2, 128), ([(1000, 1), (1000, 1)], 8, 1, 64), ([(2000, 40), (2000, 40)], 8, 1, 64),
+                                                        ([(700, 300)], 8, 1, 128), ([(513, 130), (60, 70)], 16, 2, 256), ([(400, 3)] * 70, 4, 2, 64)], ids=str)
+def test_workspace_is_enough(ctx, rows, heads, kv_heads, dim):
+    """What lies behind the workspace stays as it is: with tables just as long as the rows, also where all offsets name the same tokens."""
+    from operators_amd.ops import PagedAttentionPlan
+
+    p = Problem(rows, heads=heads, kv_heads=kv_heads, dim=dim, page=16, cache="i8", dtype="bf16", seed=1, garbage=False)
+    p.table = p.table[:, :max(-(-(a + b) // 16) for a, b in rows)].contiguous()
+    a, q = p.args(), p.q.to(DEV)
+    out = torch.full_like(q, 77.0)
+    with PagedAttentionPlan(ctx, out, q, *a, max(b for _, b in rows), p.scale) as plan:
+        size = plan.workspace_size
+        plan.workspace = torch.full((size + (16 << 20),), 0x5A, dtype=torch.uint8, device=DEV)
+        plan(out, q, *a)
+        torch.cuda.synchronize()
+        p.check(out)
+        assert (plan.workspace[size:] == 0x5A).all()
+        most = rows[0][1]
+        a[5].copy_(torch.tensor([0] + [0 if i % 2 else most for i in range(len(rows))], dtype=torch.int32))
+        a[6].fill_(2 ** 31 - 1)
+        plan(out, q, *a)
+        torch.cuda.synchronize()
+        assert (plan.workspace[size:] == 0x5A).all()

@@ -241,6 +241,23 @@ def test_attention_parameters():
     assert got == OK and 0 < size < 1 << 28
 
 
+@pytest.mark.parametrize("rows, cols, tokens, most, heads, kv, dim", [
+    (2, 2, 200, 100, 64, 8, 128), (2, 64, 200, 100, 64, 8, 128), (1, 4, 1, 1, 32, 8, 128), (1, 3, 90, 90, 8, 1, 64), (300, 8, 300, 1, 8, 1, 64), (5, 5, 40, 8, 8, 512, 256),
+    (3, 4096, 100, 100, 8, 1, 128)])
+def test_attention_workspace(rows, cols, tokens, most, heads, kv, dim):
+    """Room for no more parts than the rows' tiles can be cut into with tables of that length, nor than the GPU's units make of them."""
+    heads = max(heads, kv)
+    x = dense((tokens, heads, dim), F16)
+    got, size = create("PagedAttention", [x, x] + cache(pages=4, heads=kv, page=16, dim=dim, blocks=1) + batch(rows=rows, cols=cols), most, 0.1)
+    assert got == OK
+    steps, query, room = -(-cols * 16 // 32), most * heads // kv, 16
+    for tile, least, upto, units in ((16 if query <= 16 or dim > 128 else 32, 4 if rows == 1 else 8, 64, 4 * 256), (256 if dim <= 128 else 128, 16, query, 3 * 256)):
+        chunks = -(-steps // least)
+        slots = min(rows * -(-min(query, upto) // tile) * (chunks if chunks > 1 else 0), 2 * -(-units // kv) + 6)
+        room = max(room, slots * kv * tile * (dim + 2) * 4)
+    assert 0 < size <= room
+
+
 def test_copy_pairs():
     assert status("KVCacheCopy", cache() + [dense((7, 3), I32)]) == SHAPE
     assert status("KVCacheCopy", cache() + [dense((7, 2), torch.int64)]) == DTYPE
