@@ -16,6 +16,19 @@ constexpr uint32_t paged_unit_steps(float wanted, uint32_t least, uint32_t whole
     return ((steps < least ? least : steps) + whole - 1) & ~(whole - 1);
 }
 
+// The work and the units of many rows, added up so that no sum wraps around whatever offsets and lengths hold.  A row's tiles are
+// below 2^24 and its steps at most 2^26; of rows whose offsets name the same tokens there may be 2^24.
+struct PagedSum {
+    // Work of a workgroup's lane, at most 2^54 (of 2^9 lanes 2^63): units of that much divided among up to 2^10 are longer than any row.
+    static constexpr uint64_t work(uint64_t sum, uint64_t tiles, uint64_t steps) {
+        return sum + tiles * steps < (1ull << 54) ? sum + tiles * steps : 1ull << 54;
+    }
+    // Units in the low 48 bits, slots of the workspace (fewer than 2^16: slots_of in paged_attention_amd.cc) above.
+    static constexpr uint64_t both(uint64_t units, uint64_t slots) { return units | slots << 48; }
+    static constexpr uint64_t units(uint64_t sum) { return sum & ((1ull << 48) - 1); }
+    static constexpr uint32_t slots(uint64_t sum) { return static_cast<uint32_t>(sum >> 48); }
+};
+
 // How a call's work is cut up.  A tile is up to `tile_rows` query rows (token by
 // head of one K/V head's group) of one sequence; a unit is a tile over a range of
 // keys, and what one workgroup computes.  `target` units of a K/V head or up to three

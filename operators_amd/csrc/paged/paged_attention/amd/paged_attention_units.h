@@ -130,7 +130,7 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, uint32_t index
     uint64_t work = 0, total;
     for (uint32_t r = r0; r < r1; ++r) {
         const RowWork w = row_work(a, row_span(a.rows, r));
-        work += static_cast<uint64_t>(w.tiles) * w.steps;
+        work = PagedSum::work(work, w.tiles, w.steps);
     }
     block_scan64<WAVES>(work, slots, &total);
     const uint32_t steps = unit_steps(a, static_cast<float>(total), [&](uint32_t n) {
@@ -145,10 +145,10 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, uint32_t index
         block_scan64<WAVES>(units, slots, &sum);
         return UnitSum{static_cast<float>(sum), block_max<WAVES>(longest, slots)};
     });
-    // low half: units (JOIN: tiles of several), high half: slots of the workspace
+    // units (JOIN: tiles of several), and slots of the workspace
     const auto counts = [&](const RowWork &w, uint32_t chunks) {
         const uint64_t units = static_cast<uint64_t>(w.tiles) * chunks;
-        return (JOIN ? (chunks > 1 ? w.tiles : 0) : units) | (chunks > 1 ? units << 32 : 0);
+        return PagedSum::both(JOIN ? (chunks > 1 ? w.tiles : 0) : units, chunks > 1 ? units : 0);
     };
     uint64_t mine = 0, all;
     for (uint32_t r = r0; r < r1; ++r) {
@@ -156,15 +156,15 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, uint32_t index
         mine += counts(w, unit_chunks(w, steps));
     }
     uint64_t before = block_scan64<WAVES>(mine, slots, &all);
-    if (index >= same(static_cast<uint32_t>(all))) return false;
-    if (index >= static_cast<uint32_t>(before) && index < static_cast<uint32_t>(before + mine)) {
+    if (index >= PagedSum::units(all)) return false;
+    if (index >= PagedSum::units(before) && index < PagedSum::units(before + mine)) {
         for (uint32_t r = r0; r < r1; ++r) {
             const RowSpan s = row_span(a.rows, r);
             const RowWork w = row_work(a, s);
             const uint32_t chunks = unit_chunks(w, steps);
             const uint64_t n = counts(w, chunks);
-            if (index < static_cast<uint32_t>(before + n)) {
-                *shared = unit_of<JOIN>(a, r, s, w, chunks, index - static_cast<uint32_t>(before), static_cast<uint32_t>(before >> 32));
+            if (index < PagedSum::units(before + n)) {
+                *shared = unit_of<JOIN>(a, r, s, w, chunks, index - static_cast<uint32_t>(PagedSum::units(before)), PagedSum::slots(before));
                 break;
             }
             before += n;

@@ -183,6 +183,14 @@ def test_score_magnitudes(ctx, q_scale, new):
 
 
 @pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30, 3.0])
+def test_factors_of_the_scores(ctx, scale, new):
+    p = Problem([(700, new), (0, 3)], dim=64, cache="e4m3", dtype="f16", seed=4)
+    p.scale = scale
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("new", [1, 50])
 def test_scales_far_apart(ctx, new):
     """Blocks whose scales differ by up to 2^24, falling and rising along the row, and blocks of zeros."""
     p = Problem([(900, new)], dim=64, cache="e4m3", dtype="bf16", spread=12, q_scale=0.02, seed=3)

@@ -308,33 +308,62 @@ def test_page_table_refusals(op, args):
     assert getattr(lib, f"infiniopGet{op}WorkspaceSize")(None, None) == PARAM
 
 
+def run_cc(tmp_path, body):
+    """The lines that a host program on the library's own header prints."""
+    tu, exe = tmp_path / "one.cc", tmp_path / "one"
+    tu.write_text('#include "paged/paged_attention/amd/paged_attention_amd.h"\n#include <cstdio>\n#include <cstdlib>\n' + body)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    res = subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(ROOT, "include"), "-I", os.path.join(ROOT, "operators_amd", "csrc"),
+                          "-isystem", os.path.join(rocm, "include"), str(tu), "-o", str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    return lambda *args: subprocess.run([str(exe), *map(str, args)], capture_output=True, text=True, check=True).stdout.split()
+
+
 @pytest.mark.skipif(shutil.which("g++") is None, reason="no C++ compiler")
 def test_units_of_rows_that_are_long_together(tmp_path):
     """How long a unit of attention is, as the kernels work it out, where the rows' steps exceed 2^32 together: 64 rows of 2^31 places
     and one unit to be made of each of 256 K/V heads.  A number that wrapped around would cut them into more units than the grid
     and the workspace have room for."""
-    tu, exe = tmp_path / "steps.cc", tmp_path / "steps"
-    tu.write_text('''#include "paged/paged_attention/amd/paged_attention_amd.h"
-#include <cstdio>
-#include <cstdlib>
-int main(int n, char **v) {
+    unit_steps = run_cc(tmp_path, '''int main(int n, char **v) {
     for (int i = 1; i + 2 < n; i += 3) std::printf("%u\\n", paged_unit_steps(std::strtof(v[i], nullptr), std::atoi(v[i + 1]), std::atoi(v[i + 2])));
 }
 ''')
-    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-    res = subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(ROOT, "include"), "-I", os.path.join(ROOT, "operators_amd", "csrc"),
-                          "-isystem", os.path.join(rocm, "include"), str(tu), "-o", str(exe)], capture_output=True, text=True)
-    assert res.returncode == 0, res.stderr
     wanted = [0.0, 0.5, 7.0, 15.9, 16.0, 100.5, 2.0 ** 20, 2.0 ** 26, 2.0 ** 29 + 64, 2.0 ** 30, 2.0 ** 31, 2.0 ** 32 - 256, 2.0 ** 32, 1.5 * 2.0 ** 32, 2.0 ** 40, 1e30]
     for least, whole in ((4, 1), (8, 1), (16, 2)):
-        out = subprocess.run([str(exe)] + [str(x) for w in wanted for x in (w, least, whole)], capture_output=True, text=True, check=True).stdout.split()
+        out = unit_steps(*[x for w in wanted for x in (w, least, whole)])
         for w, steps in zip(wanted, map(int, out)):
             assert steps >= least and steps % whole == 0 and steps >= min(w, 2 ** 30) and steps <= max(w + 2, least, 2) and steps <= 2 ** 30, (w, steps)
     total, longest = 64 * 2 ** 26, 2 ** 26
     for by in (1.5, 1.25, 1.0, 2 / 3, 0.5, 1 / 3):
-        out = int(subprocess.run([str(exe), str(total * by * 1.00001), "16", "2"], capture_output=True, text=True, check=True).stdout)
+        out = int(unit_steps(total * by * 1.00001, 16, 2)[0])
         units = 64 * -(-longest // out)
         assert units <= 64 + total / (total * by) and (units == 64 or units <= 2 * total / (total * by)), by
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no C++ compiler")
+def test_sums_over_rows_that_name_the_same_tokens(tmp_path):
+    """Offsets that rise and fall again give half of all rows all tokens.  131072 such rows of 32768 tiles are 2^32 units, 2^24 rows of
+    nearly 2^24 tiles of 2^26 steps more work than 64 bits hold: no sum of units reaches that of the slots, and no sum of work wraps."""
+    sums = run_cc(tmp_path, '''int main() {
+    uint64_t all = 0;
+    for (int lane = 0; lane < 512; ++lane) {
+        uint64_t mine = 0;
+        for (int r = 0; r < 256; ++r) mine += PagedSum::both(32768, 0);
+        all += mine;
+    }
+    all += PagedSum::both(7, 1535);
+    std::printf("%llu %u\\n", (unsigned long long)PagedSum::units(all), PagedSum::slots(all));
+    uint64_t total = 0;
+    for (int lane = 0; lane < 512; ++lane) {
+        uint64_t mine = 0;
+        for (int r = 0; r < 32768; ++r) mine = PagedSum::work(mine, (1u << 24) - 1, 1u << 26);
+        total += mine;
+    }
+    std::printf("%llu\\n", (unsigned long long)total);
+    std::printf("%llu %llu\\n", (unsigned long long)PagedSum::work(5, 3, 1000), (unsigned long long)PagedSum::work((1ull << 54) - 1, 1, 1));
+}
+''')
+    assert [int(x) for x in sums()] == [2 ** 32 + 7, 1535, 2 ** 63, 3005, 2 ** 54]
 
 
 def test_no_fallback():
