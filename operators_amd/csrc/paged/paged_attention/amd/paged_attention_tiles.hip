@@ -149,9 +149,9 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         asm volatile("" : "+v"(v));
         return v;
     };
-    const auto page_of = [&](uint32_t tile) {
+    const auto page_of = [&](uint32_t tile, uint32_t upto) {// (upto: below it a key has to lie)
         const uint32_t key = first_key + tile * BK + seldom(lane) * 16;
-        if (key >= u.length) return -1;
+        if (key >= upto) return -1;
         const int page = table[fast_quotient(key, a.rows.by_page)];
         return static_cast<uint32_t>(page) < a.pages ? page : -1;
     };
@@ -168,18 +168,18 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     };
     uint64_t k_group, v_group, v_none, v_none_before;// v_none: a bit for each group without a page, of this set and the last
     {
-        const int page = page_of(0);
+        const int page = page_of(0, u.length);
         k_group = bytes_of(0, page, a.k_at);
         v_group = bytes_of(0, page, a.v_at);
         v_none = v_none_before = __builtin_amdgcn_ballot_w64(page < 0);
     }
     const auto k_set = [&](uint32_t tile) {
-        if (tile % kAhead == 0) k_group = bytes_of(tile, page_of(tile), a.k_at);
+        if (tile % kAhead == 0) k_group = bytes_of(tile, page_of(tile, u.length), a.k_at);
     };
     const auto v_set = [&](uint32_t tile) {
         v_none_before = v_none;
         if (tile % kAhead == 0) {
-            const int page = page_of(tile);
+            const int page = page_of(tile, u.length);
             v_group = bytes_of(tile, page, a.v_at);
             v_none = __builtin_amdgcn_ballot_w64(page < 0);
         }
@@ -321,13 +321,13 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
     float k_scale, v_rel, v_back;// of the lane's group: of V log2 relative to v_top, and the way back
     uint64_t no_page = 0;        // a bit for each group
     const auto scales = [&](uint32_t tile) {
-        const int page = page_of(tile);
+        const int page = page_of(tile, some_see);// (what none of these rows sees counts as no page)
         float v_log = kZeroScale;
         k_scale = 0.0f;
         if (page >= 0) {
-            const uint32_t key = first_key + tile * BK + seldom(lane) * 16, block = fast_quotient(place_of(key), a.by_block);
+            const uint32_t block = fast_quotient(place_of(first_key + tile * BK + seldom(lane) * 16), a.by_block);
             k_scale = ks_base[page * a.k_at.s_page + block];
-            if (key < some_see) v_log = fmaxf(log2_of(vs_base[page * a.v_at.s_page + block]), kZeroScale);
+            v_log = fmaxf(log2_of(vs_base[page * a.v_at.s_page + block]), kZeroScale);
         }
         asm volatile("" : "+v"(k_scale));// (waited for here, not where this way and the one past it meet)
         no_page = __builtin_amdgcn_ballot_w64(page < 0);
@@ -369,13 +369,14 @@ __global__ __launch_bounds__(paged_tile_waves(DP) *kWave) void paged_attention_t
         const uint32_t at = tile % kAhead * NG;
         high = kNone;
 #pragma unroll
+        for (int g = 0; g < NG; ++g) rel[g] = lane_of(v_rel, at + g);
+#pragma unroll
         for (int g = 0; g < NG; ++g) {
             // (above 0, so that what is not seen stays at minus infinity)
             f[g] = fmaxf(factor * lane_of(k_scale, at + g), 0x1p-126f);
             const f32x16 &x = s[g / 2];
             const int b = g % 2 * 8;
             const float top = fmaxf(fmaxf(fmaxf(fmaxf(x[b], x[b + 1]), x[b + 2]), fmaxf(fmaxf(x[b + 3], x[b + 4]), x[b + 5])), fmaxf(x[b + 6], x[b + 7]));
-            rel[g] = lane_of(v_rel, at + g);
             high = fmaxf(high, __builtin_fmaf(top, f[g], rel[g]));
         }
     };

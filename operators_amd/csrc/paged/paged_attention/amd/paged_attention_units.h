@@ -176,10 +176,9 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, uint32_t index
     return true;
 }
 
-// log2, of subnormal numbers too, which the instruction takes as 0; minus infinity of 0.
+// log2, of subnormal numbers too, which the instruction by itself takes as 0; minus infinity of 0.
 __device__ __forceinline__ float log2_of(float v) {
-    const bool low = v < 0x1p-100f;
-    return __builtin_amdgcn_logf(low ? v * 0x1p100f : v) - (low ? 100.0f : 0.0f);
+    return __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(v)) + static_cast<float>(__builtin_amdgcn_frexp_expf(v));
 }
 // A unit's weight beside others': l relative to 2^m, several of them together.
 struct Weight {
