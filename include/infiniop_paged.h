@@ -88,9 +88,9 @@ INFINIOP_C INFINIOP_EXPORT infiniopStatus_t infiniopDestroyKVCacheAppendDescript
  * usually 1 / sqrt(dim).  q and what the cache holds for a row's places have to
  * be finite, and so has scale * q K in fp32; behind lengths[r] it may hold anything.
  * Scores, sums and results are fp32 (rounded once, to nearest even); q is rounded to
- * fp16 relative to the largest of its row, which is exact but for elements 2^-24 of it
- * and less, and the weights, each times its V scale, to fp16 (11 bits) relative to the
- * largest of the same query row.  In chunks of many tokens a V scale below 2^-80 of the
+ * fp16 relative to the largest element of its row, by at most 2^-25 of that, and the
+ * weights, each times its V scale, to fp16 (11 bits, none below 2^-35 of the largest of
+ * the same query row).  In chunks of many tokens a V scale below 2^-80 of the
  * largest that neighbouring tokens see may count as 2^-80 of that.
  * ======================================================================== */
 typedef struct PagedAttentionDescriptor {

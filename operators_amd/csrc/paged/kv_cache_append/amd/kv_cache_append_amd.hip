@@ -6,9 +6,10 @@
 // scale belongs to exactly one of them: no two wavefronts share a number, and the
 // result does not depend on their order.  The power of two makes rescaling e4m3
 // codes exact but for what sinks below its smallest normal number.
-// Bound by HBM for prompts (2 bytes read, 1 written per value: 8500 tokens of 8 heads x
-// 128 13.7 us, 3.8 TB/s; a large element-wise pass reaches 6.2), by the chain
-// table -> codes for a few tokens (256 rows of one 5.6 us).
+// Prompts: 2 bytes read, 1 written per value, 8500 tokens of 8 heads x 128 12.7 us, 4.1 TB/s
+// where a large element-wise pass reaches 6.2: all workgroups are one round, begin by looking
+// for their units, then load, then store, and nothing of one overlaps another.  A few
+// tokens: the chain table -> codes (256 rows of one 5.7 us).
 #include "../../paged_kernel.h"
 #include "kv_cache_append_amd.h"
 
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(kAppendWaves *kWave) void kv_cache_append(AppendArg
 }
 
 // Decoding: where tokens are not many more than rows, a workgroup for each token looks its row up, without the scan
-// over all rows that gives the units of long prompts (256 rows of a token, 8 heads x 128: 8.3 us with the scan, 5.6
+// over all rows that gives the units of long prompts (256 rows of a token, 8 heads x 128: 8.3 us with the scan, 5.7
 // without).  Beyond 1024 rows the look takes longer than the scan.
 bool by_token(const KVCacheAppendAmdDescriptor &d) { return d.tokens <= 2ull * d.rows.rows && d.rows.rows <= 1024; }
 

@@ -2,9 +2,10 @@
 //     rows:    row r := row source[r]; refcount[p] += rows that got p - rows that gave it up
 //     growth:  need[r] = pages(length + grow) - pages(length) + (1 if the last page is shared and grows)
 //     fresh:   the k-th free page goes to the row whose need covers k in the running sum
-// Four phases, each of which needs all of the one before: (1) the rows that change
-// are laid aside, (2) counts, (3) free pages marked and counted, needs worked out,
-// rows written, (4) fresh pages handed out.  Whole numbers throughout, added by
+// Four phases: (1) the rows that change are laid aside, (2) counts, (3) free pages marked
+// and counted, needs worked out, rows written, (4) fresh pages handed out.  (3) and (4)
+// need all of the one before, (2) of (1) the copy of the counts, where they go
+// elsewhere, and of the rows its own.  Whole numbers throughout, added by
 // atomics whose order does not matter.  Latency bound.  A launch for each phase, or, where
 // the table fits the registers and the counts the LDS of one workgroup, all of them in
 // one launch with three waits for memory (64 rows of 64, 4096 pages: 15.3 us in four

@@ -65,7 +65,9 @@ infiniopStatus_t amdCreatePagedAttentionDescriptor(AmdHandle_t handle, PagedAtte
     const uint64_t busy = rows.rows < tokens ? rows.rows : tokens, query_rows = tokens * group, most_rows = max_tokens * group;
     const uint64_t cus = static_cast<uint64_t>(handle->cu_count);
     PagedAttentionShape few{}, many{};
-    // two sets of 16 rows share what they read; heads wider than 128 leave no registers for that
+    // two sets of 16 rows share what they read; heads wider than 128 leave no registers for that.  (us with tiles of 32 and of 16 rows,
+    // 64/8 heads x 128, 32 rows of 8192 keys: 4 new tokens 123 and 172, 8 193 and 285; a call with a chunk of a prompt gives its single
+    // tokens half-empty tiles: 8 beside a chunk of 500, 40/8 x 80, 253 and 246, 99 beside one of 600, 64/8 x 128, 285 and 272)
     few.tile_rows = most_rows <= 16 || cache.dim > 128 ? 16 : 32;
     few.least = 1;
     few.most = kFewRows;

@@ -8,8 +8,8 @@
 // between lanes.  For V a lane holds the same 8 keys of dim / 16 neighbouring
 // columns: byte permutations turn 8 keys x 4 columns round in registers.
 // Codes are exact in fp16; q is multiplied by a power of two for each row that
-// brings its largest element to [1, 2), so that it is too (but for what is 2^24 times
-// smaller than that element), whatever its type.  Scores, maxima, sums and O are fp32.
+// brings its largest element to [1, 2), so that it is off by at most 2^-25 of that
+// element, whatever its type.  Scores, maxima, sums and O are fp32.
 // The scale of a V block goes into P, whose running maximum is its own: with m_o of
 // score + log2(V scale) and m of the scores,
 //     P = exp2(score + log2(V scale) - m_o),  l = sum(exp2(score - m)),  out = V^T P 2^(m_o - m) / l
@@ -23,7 +23,7 @@
 // leaves the usual step without an exchange between lanes.
 // Bound by reading K and V once from HBM: 64 heads on 8 of 128 columns, 48 sequences of
 // 100 to 131072 keys 347 us (5.5 TB/s; a large element-wise pass reaches 6.2), one of 131072
-// 52 us (5.1), one of 1000 10.7 us, which is two launches and four waits for memory in turn.
+// 51 us (5.2), one of 1000 11 us, which is two launches and four waits for memory in turn.
 #include "paged_attention_units.h"
 
 namespace {

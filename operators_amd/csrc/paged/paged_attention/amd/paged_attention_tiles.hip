@@ -19,14 +19,14 @@
 // Two wavefronts share a SIMD and are a phase apart: one at its products, the other at
 // its exponentials and the next tile's codes (when that took 330 us in the example
 // below: 353 without, 390 with wavefronts of the same phase on a SIMD).
-// 64 heads on 8 of 128 columns, a prompt of 4096 tokens: 309-318 us, 0.88 PFLOP/s; a
-// library product of large fp16 matrices reaches 1.34.  Of that time (at 2.0 GHz) the
-// matrix units are at work 40 %, the vector units 55 % (7 slots for each score, 4 of
-// them the exponential), LDS 30 %.  Without the products the rest takes 231 us, without
-// the tiles' way from memory into LDS 300: bound by how far a SIMD does products and vector
-// instructions of two wavefronts at once, and by the barrier after each phase.  Heads of
-// 256 columns, 32 on 8, 2048 tokens: 168 us, 0.41 PFLOP/s, for one wavefront a SIMD
-// overlaps nothing.
+// 64 heads on 8 of 128 columns, a prompt of 4096 tokens: 291-318 us (from GPU to GPU), 0.9
+// PFLOP/s; a library product of large fp16 matrices reaches 1.34.  Of that time (at 2.0 GHz)
+// the matrix units are at work 40 %, the vector units 57 % (7 slots for each score, 4 of
+// them the exponential), LDS 30 %.  Where the whole took 310 us, it took 231 without the products
+// and 300 without the tiles' way from memory into LDS: bound by how far a SIMD does products and
+// vector instructions of two wavefronts at once, and by the barrier after each phase.  Heads of
+// 256 columns, 32 on 8, 2048 tokens: 169 us, 0.41 PFLOP/s; one wavefront a SIMD does its
+// products and its exponentials one after the other.
 #include "paged_attention_units.h"
 
 namespace {
