@@ -799,7 +799,19 @@ def main():
         out["cpu_baseline"] = cpu_baseline(T)
         if not args.no_ops_table:
             attach_cpu(out["ops"], cpu_per_op(T))
-    print(json.dumps(out))
+    if "ops" in out:
+        print(json.dumps({"ops": out["ops"]}), file=sys.stderr)
+    print(result_line(out))
+
+
+# The one line on stdout has to stay short for those who read it back from the end of a log: of each row of the per-operator
+# table it holds the figure and the fraction, the whole table goes to stderr.
+LINE_KEYS = ("config", "us_per_call", "frac_of_peak")
+
+
+def result_line(out):
+    rows = [{k: r[k] for k in LINE_KEYS if k in r} for r in out.get("ops", [])]
+    return json.dumps({**out, "ops": rows} if rows else out, separators=(",", ":"))
 
 
 # Rows of the per-operator table whose figures also go, as flat scalars, into `config`

@@ -94,6 +94,23 @@ def test_xmake_file_names_the_gfx950_option():
     assert "cuda" not in text.lower().replace("no cuda headers", "")
 
 
+def test_bench_prints_a_short_line():
+    """The result stays one JSON object of less than 8 KiB however much the per-operator table holds of each of its rows."""
+    import json
+    import sys
+
+    sys.path.insert(0, ROOT)
+    import bench
+
+    row = {"op": "rearrange", "config": "x" * 60, "us_per_call": 12345.678, "frac_of_peak": 0.1234, **{f"field_{i}": 1234567.8 for i in range(20)}}
+    out = {"metric": "m", "value": 6536.5, "config": {f"frac_{i}": 0.1234 for i in range(60)}, "roofline": {f"k{i}": 1.5 for i in range(12)}, "ops": [row] * 45}
+    line = bench.result_line(out)
+    got = json.loads(line)
+    assert "\n" not in line and len(line) < 8192
+    assert got["value"] == 6536.5 and got["ops"][0] == {"config": "x" * 60, "us_per_call": 12345.678, "frac_of_peak": 0.1234} and len(got["ops"]) == 45
+    assert json.loads(bench.result_line({"metric": "m", "value": 1.0})) == {"metric": "m", "value": 1.0}
+
+
 def test_bench_reads_its_traffic_figure_from_the_committed_profile(tmp_path):
     """roofline.traffic is the swiglu row of profiles/c5_kernels_hbm_traffic_pmc.txt, byte for byte, and its absence is an error."""
     import sys
